@@ -86,6 +86,14 @@ PROTOTYPES = {
     "exl3r_rope_paged_kv_had": (_i, [_vp, _vp, _i64, _i, _vp, _vp, _i64, _vp, _i64, _i, _i, _i64, _i64, _i, _vp, _i,
                                      _i32, _vp, _vp, _vp, _vp, _i, _f, _f, _i, _f, _vp, _vp, _i, _i64,
                                      _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "exl3r_paged_attn": (_i, [_vp, _i64, _i64, _i, _vp, _vp, _i, _i, _i64, _vp, _i64, _vp, _i, _i64, _i64, _i, _f, _i, _i,
+                              _vp, _i64, _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "exl3r_paged_attn_shared": (_i, [_vp, _i64, _i64, _i, _vp, _vp, _i, _i, _i64, _vp, _i64, _vp, _i64, _i, _i64, _i64, _i,
+                                     _f, _i, _i, _vp, _i64, _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "exl3r_paged_attn_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i, _i, _i, _i, _i64, _i64]),
+    "exl3r_token_logprobs": (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                                  _vp]),
+    "exl3r_token_logprobs_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "exl3r_embedding": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _vp]),
     "exl3r_embedding_rms_norm": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i, _i64, _vp, _i, _i64, _vp, _i,
                                       _vp, _i, _i64, _f, _f, _f, _vp, _vp]),

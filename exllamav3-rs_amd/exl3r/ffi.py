@@ -11,6 +11,7 @@ The wrappers of a forward pass hand their arguments to the native module first (
 which makes the call or declines it; what follows in the wrapper is the general form and has the errors.  A
 decode layer's four calls took 42.8 us through ctypes and take 14.6 through the native module; the GPU needs
 11.8 us for them (one graph of the four), so such a layer is still bound by its host calls."""
+import contextlib
 import ctypes
 import math
 
@@ -37,6 +38,11 @@ def _stream(t, stream):
     if stream is not None:
         return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _on(t):
+    """The tensor's device as the current one (a launch goes to the current device's code)."""
+    return torch.cuda.device(t.device) if t.is_cuda else contextlib.nullcontext()
 
 
 def _rows(t):
@@ -610,6 +616,122 @@ def gumbel_noise(x, out, random=0, stream=None):
         raise ValueError("x and out must have the same shape")
     check(load().exl3r_gumbel_noise(_ptr(x), dtype_code(x), ldx, _ptr(out), dtype_code(out), ldo, rows, cols,
                                     int(random) & 0xFFFFFFFF, _stream(x, stream)))
+
+
+def _ws_args(ws, like):
+    """(pointer, bytes) of an optional workspace tensor; the C ABI says what it has to hold."""
+    if ws is None:
+        return None, 0
+    if ws.device != like.device or not ws.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the inputs' device")
+    return _ptr(ws), ws.numel() * ws.element_size()
+
+
+def paged_attn_workspace_bytes(q, k_cache, block_table, shared_len=0):
+    """Bytes of the workspace that paged_attn (or paged_attn_shared with this shared_len) takes for these shapes."""
+    bsz, seq, hq, hd = q.shape
+    return int(load().exl3r_paged_attn_workspace_bytes(bsz, seq, hq, k_cache.shape[2], hd, k_cache.shape[1],
+                                                       block_table.shape[1], int(shared_len)))
+
+
+def _paged_attn(shared_len, q, k_cache, v_cache, block_table, cache_seqlens, out, scale, window, sinks, lse, workspace,
+                err_flag, stream):
+    if q.dim() != 4 or out.shape != q.shape:
+        raise ValueError("q and out must be (bsz, seq_len, heads, head_dim)")
+    bsz, seq, hq, hd = q.shape
+    for t in (q, out):
+        if t.numel() and (t.stride(3) != 1 or (seq > 1 and bsz > 1 and t.stride(0) != seq * t.stride(1))):
+            raise ValueError("q / out: dense innermost dim and batch stride seq_len * token stride")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != hd or not k_cache.is_contiguous() or \
+            not v_cache.is_contiguous():
+        raise ValueError("caches must be contiguous (pages, page_size, kv_heads, head_dim)")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype or out.dtype != q.dtype:
+        raise TypeError("q, out and the caches must share a dtype")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or cache_seqlens.dtype != torch.int32:
+        raise TypeError("block_table (bsz, max_blocks) and cache_seqlens (bsz) must be int32")
+    if block_table.shape[0] != bsz or cache_seqlens.numel() != bsz or not block_table.is_contiguous() or \
+            not cache_seqlens.is_contiguous():
+        raise ValueError("block_table and cache_seqlens must be contiguous with one row / entry per sequence")
+    if lse is not None and (lse.dtype != torch.float32 or lse.numel() != bsz * seq * hq or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 (bsz, seq_len, heads)")
+    if err_flag is not None and err_flag.dtype != torch.int32:
+        raise TypeError("err_flag must be int32")
+    for t in (k_cache, v_cache, block_table, cache_seqlens, out, lse, err_flag):
+        if t is not None and t.device != q.device:
+            raise ValueError("every tensor must be on the device of q")
+    # a batch of one-token sequences may lie at any batch stride
+    qs, os = (t.stride(0) if seq == 1 else t.stride(1) for t in (q, out))
+    wp, wb = _ws_args(workspace, q)
+    args = [_ptr(q), qs, q.stride(2), hq, _ptr(k_cache), _ptr(v_cache), k_cache.shape[2], k_cache.shape[1],
+            k_cache.shape[0], _ptr(block_table), block_table.shape[1], _ptr(cache_seqlens)]
+    rest = [dtype_code(q), bsz, seq, hd, 1.0 / math.sqrt(hd) if scale is None else float(scale), int(window), int(sinks),
+            _ptr(out), os, out.stride(2), _ptr(lse), _ptr(err_flag), wp, wb]
+    with _on(q):
+        if shared_len is None:
+            check(load().exl3r_paged_attn(*args, *rest, _stream(q, stream)))
+        else:
+            check(load().exl3r_paged_attn_shared(*args, int(shared_len), *rest, _stream(q, stream)))
+
+
+def paged_attn(q, k_cache, v_cache, block_table, cache_seqlens, out, scale=None, window=0, sinks=0, lse=None,
+               workspace=None, err_flag=None, stream=None):
+    """Causal attention of q (bsz, seq_len, heads, head_dim) over the paged caches that rope_paged_kv filled, called
+    after it with the same block_table and cache_seqlens: token s of sequence b, at position cache_seqlens[b] + s, sees
+    the positions up to its own, with window > 0 only the last `window` of them and the first `sinks`.  scale None:
+    1 / sqrt(head_dim).  lse: float32 (bsz, seq_len, heads), the scores' log-sum-exp.  workspace: a uint8 tensor of
+    paged_attn_workspace_bytes() bytes (any contents; not shared by calls that overlap)."""
+    _paged_attn(None, q, k_cache, v_cache, block_table, cache_seqlens, out, scale, window, sinks, lse, workspace, err_flag,
+                stream)
+
+
+def paged_attn_shared(q, k_cache, v_cache, block_table, cache_seqlens, out, shared_len, scale=None, window=0, sinks=0,
+                      lse=None, workspace=None, err_flag=None, stream=None):
+    """paged_attn of a batch whose sequences have their first shared_len positions (whole pages) on the same pages:
+    those keys are read once for the whole batch.  The block table's rows must agree there (row 0's entries are read)."""
+    _paged_attn(shared_len, q, k_cache, v_cache, block_table, cache_seqlens, out, scale, window, sinks, lse, workspace,
+                err_flag, stream)
+
+
+def token_logprobs_workspace_bytes(rows, vocab):
+    """Bytes of the workspace that token_logprobs takes for logits of this shape."""
+    return int(load().exl3r_token_logprobs_workspace_bytes(rows, vocab))
+
+
+def token_logprobs(logits, tokens, logprobs, entropy=None, top_ids=None, top_logprobs=None, max_logit=0, workspace=None,
+                   err_flag=None, stream=None):
+    """logprobs[i] = log softmax(logits[i, :max_logit])[tokens[i]] (tokens and logprobs may both be None), entropy[i] that
+    distribution's entropy, and its top_ids.shape[-1] most probable tokens, ties to the lowest id, with their log
+    probabilities, in one read of the logits.  float32 outputs, int64 ids.  workspace: a uint8 tensor of
+    token_logprobs_workspace_bytes() bytes (any contents; not shared by calls that overlap)."""
+    rows, vocab, ld = _rows(logits)
+    k = 0
+    if (tokens is None) != (logprobs is None):
+        raise ValueError("tokens and logprobs go together")
+    if tokens is not None and (tokens.dtype != torch.int64 or tokens.numel() != rows or not tokens.is_contiguous()):
+        raise ValueError("tokens must be int64 with one entry per row")
+    for t in (logprobs, entropy):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != rows or not t.is_contiguous()):
+            raise ValueError("logprobs and entropy must be float32 with one entry per row")
+    if (top_ids is None) != (top_logprobs is None):
+        raise ValueError("top_ids and top_logprobs go together")
+    if top_ids is not None:
+        if top_ids.dim() == 0 or top_ids.shape != top_logprobs.shape or top_ids.dtype != torch.int64 or \
+                top_logprobs.dtype != torch.float32 or not top_ids.is_contiguous() or not top_logprobs.is_contiguous():
+            raise ValueError("top_ids (int64) and top_logprobs (float32) must be contiguous [rows, k]")
+        k = top_ids.shape[-1]
+        if top_ids.numel() != rows * k:
+            raise ValueError("top_ids must hold one row per row of logits")
+    if err_flag is not None and err_flag.dtype != torch.int32:
+        raise TypeError("err_flag must be int32")
+    for t in (tokens, logprobs, entropy, top_ids, top_logprobs, err_flag):
+        if t is not None and t.device != logits.device:
+            raise ValueError("every tensor must be on the device of the logits")
+    wp, wb = _ws_args(workspace, logits)
+    with _on(logits):
+        check(load().exl3r_token_logprobs(_ptr(logits), dtype_code(logits), rows, vocab, ld, int(max_logit), _ptr(tokens),
+                                          _ptr(logprobs), _ptr(entropy), k, _ptr(top_ids) if k else None,
+                                          _ptr(top_logprobs) if k else None, _ptr(err_flag), wp, wb,
+                                          _stream(logits, stream)))
 
 
 def had_r_128(x, out, pre_scale=None, post_scale=None, scale=1.0, stream=None, mfma=False):

@@ -599,6 +599,81 @@ EXL3R_API int exl3r_act_mul_had(int act, const void* x, const void* y, int in_dt
                       const void* x_post_scale, const void* y_post_scale, void* stream);
 
 /*
+ * Causal attention over the paged KV cache that exl3r_rope_paged_kv fills, with an optional sliding window whose
+ * first tokens ("sinks") stay visible.  Called after the append, with the same cache_seqlens: token s of sequence b
+ * is at position p = cache_seqlens[b] + s (int32 [bsz], device) and sees the keys j with 0 <= j <= p and
+ * (window <= 0, or p - j < window, or j < sinks):
+ *   out[b, s, h] = sum_j w_j v_j, w = softmax over the visible j of scale * q[b, s, h] . k_j;
+ *   lse[b, s, h] = ln sum_j exp(scale * q . k_j)  (float32 [bsz * seq_len, num_heads_q]; lse == NULL: not written).
+ * Scores, softmax and sums in fp32 (a weight is rounded to dtype as the second product's operand); out is rounded
+ * once.  A token that sees nothing has out 0 and lse -inf.  Values of keys that a token does not see reach its
+ * result in no way, infinities and NaNs included.  No counterpart in this path's reference files: its attention
+ * is the flash / paged call between paged_kv_cache_update and o_proj (src/modules.rs:704-787).
+ *   q:   [bsz, seq_len, num_heads_q, head_dim] of dtype (F16/BF16): element (b, s, h, d) at
+ *        (b*seq_len + s)*q_tok_stride + h*q_head_stride + d; out likewise with its own strides (out == q with equal
+ *        strides is allowed).  head_dim 64, 128 or 256; num_heads_q a multiple of num_heads_kv, query head h
+ *        reading KV head h / (num_heads_q / num_heads_kv).
+ *   k_cache, v_cache, page_size, num_pages, block_table, max_blocks_per_seq: as exl3r_rope_paged_kv (16-byte
+ *        aligned).  max_blocks_per_seq * page_size below 2^31.
+ *   err_flag: NULL or a device int32; 1 is stored for a token whose position is negative or past its block table
+ *        (it sees the keys that the table holds) and for a visible key whose page is outside [0, num_pages) (it is
+ *        taken as not visible).
+ *   scale: positive and finite (1 / sqrt(head_dim) as a rule).  sinks must be 0 without a window.
+ *   workspace: exl3r_paged_attn_workspace_bytes() bytes of device memory, 256-byte aligned (NULL where that is 0),
+ *        for the partial results of long key ranges cut over workgroups.  It needs no initial value and keeps none;
+ *        calls that share one must not overlap.
+ */
+EXL3R_API int exl3r_paged_attn(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int num_heads_q,
+                     const void* k_cache, const void* v_cache, int num_heads_kv, int page_size, int64_t num_pages,
+                     const int32_t* block_table, int64_t max_blocks_per_seq, const int32_t* cache_seqlens,
+                     int dtype, int64_t bsz, int64_t seq_len, int head_dim, float scale, int window, int sinks,
+                     void* out, int64_t out_tok_stride, int64_t out_head_stride, float* lse, int32_t* err_flag,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * exl3r_paged_attn for a batch whose sequences share a prefix: the first shared_len positions (a whole number of
+ * pages) of every sequence are on the same pages, block_table[b][0 .. shared_len / page_size) being equal for all b
+ * (sequence 0's entries are read).  Their keys are then read once for the query rows of the whole batch instead of
+ * once per sequence.  Every other argument, and the result up to the order of the sums, as exl3r_paged_attn.
+ * shared_len 0 is exl3r_paged_attn.
+ */
+EXL3R_API int exl3r_paged_attn_shared(const void* q, int64_t q_tok_stride, int64_t q_head_stride, int num_heads_q,
+                            const void* k_cache, const void* v_cache, int num_heads_kv, int page_size,
+                            int64_t num_pages, const int32_t* block_table, int64_t max_blocks_per_seq,
+                            const int32_t* cache_seqlens, int64_t shared_len, int dtype, int64_t bsz, int64_t seq_len,
+                            int head_dim, float scale, int window, int sinks, void* out, int64_t out_tok_stride,
+                            int64_t out_head_stride, float* lse, int32_t* err_flag, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that suffice for these calls at any window (0 for shapes they refuse, and where none is used);
+ * shared_len 0 for exl3r_paged_attn. */
+EXL3R_API size_t exl3r_paged_attn_workspace_bytes(int64_t bsz, int64_t seq_len, int num_heads_q, int num_heads_kv,
+                                                  int head_dim, int page_size, int64_t max_blocks_per_seq,
+                                                  int64_t shared_len);
+
+/*
+ * Log probabilities of given tokens, the entropy and the most probable tokens of logits rows, in one read of them:
+ *   z = ln sum_c exp(x[r, c]) over the columns c < n (n = max_logit, or vocab where max_logit <= 0 or > vocab);
+ *   logprobs[r] = x[r, tokens[r]] - z;   entropy[r] = -sum_c P_c ln P_c, P_c = exp(x[r, c] - z);
+ *   top_ids[r, i], top_logprobs[r, i]: the top_k largest logits' columns in falling order, equal ones by rising
+ *   column (exl3r_argmax_sample's order: NaN largest, -0 equal to +0), and their log probabilities.
+ * fp32 with the row's sums joined in fp64.  Columns from max_logit on are masked out as in exl3r_argmax_sample.  A
+ * token outside [0, n) has log probability -inf; one outside [0, vocab) also stores 1 to *err_flag (device int32, or
+ * NULL).  A NaN or +inf among a row's logits, or all of them -inf, make its results NaN (top_ids stay defined).
+ *   logits: [rows, vocab], row stride ld elements, F16/BF16/F32.  tokens: int64 [rows], or NULL: logprobs is not
+ *        written (and may be NULL).  logprobs, entropy: float32 [rows] or NULL.  top_k: 0 (top_ids, top_logprobs
+ *        NULL) to 32, at most n; top_ids int64 and top_logprobs float32 [rows, top_k].
+ *   workspace: exl3r_token_logprobs_workspace_bytes() bytes, 256-byte aligned, uninitialised; calls that share one
+ *        must not overlap.
+ * No counterpart in the reference; for the callers of exl3r_argmax_sample and exl3r_gumbel_sample that report what
+ * they drew, and for scoring given text.
+ */
+EXL3R_API int exl3r_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, int max_logit,
+                         const int64_t* tokens, float* logprobs, float* entropy, int top_k, int64_t* top_ids,
+                         float* top_logprobs, int32_t* err_flag, void* workspace, size_t workspace_bytes, void* stream);
+EXL3R_API size_t exl3r_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab);
+
+/*
  * Token-embedding gather: out[i, :] = table[ids[i], :], bit-exact (same dtype) or exactly upcast to
  * F32.  Replaces Embedding::forward's index_select + to_kind(Float) (src/modules.rs:430-436).
  *   table: [vocab, hidden], row stride ldt, F16/BF16/F32.
