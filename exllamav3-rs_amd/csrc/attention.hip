@@ -24,6 +24,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 template <class T> using lptr = __attribute__((address_space(3))) T*;
 
+constexpr int kMaxSplits = 512;      // of a row: 256 of the shared prefix and 256 of its own keys
+
 struct AttnArgs
 {
     const char* q;
@@ -34,8 +36,8 @@ struct AttnArgs
     const int32_t* table;
     const int32_t* lens;
     int32_t* err;
-    float* po;                // partial outputs [split][row][HD], unnormalised
-    float* pml;               // ... and their {c m - shift, l} [split][row][2]
+    float* po;                // partial outputs [row][split][HD], unnormalised
+    float* pml;               // ... and their {c m - shift, l} [row][split][2]
     int64_t q_ts, q_hs, o_ts, o_hs;     // elements
     int64_t max_blocks, num_pages;
     int64_t rows_all;         // bsz * seq * hq
@@ -43,7 +45,7 @@ struct AttnArgs
     int32_t page_shift, window, sinks;
     int32_t dom_lo, dom_hi;   // keys of this launch: [dom_lo, dom_hi)
     int32_t rows;             // query rows per row set (a sequence's, or the whole batch's)
-    int32_t row_tiles, nsplit, split0;
+    int32_t row_tiles, nsplit, split0, splits;   // this launch's splits, their first place among all `splits`
     int32_t whole;            // 1: one row set of all sequences, keys through sequence 0's table row
     int32_t direct;           // 1: this launch's result is the output
     int32_t q_vec, o_vec;     // 16-byte aligned q rows / 8-byte aligned out rows
@@ -60,6 +62,15 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
 }
 
 template <class IO>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c)
+{
+    if constexpr (IO::code == DT_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <class IO>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi)
 {
     if constexpr (IO::code == DT_F16) return pack_f16(lo, hi);
@@ -71,6 +82,14 @@ __device__ __forceinline__ float max_xor32(float v)
 {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
     const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
+}
+
+// ... of the four lanes l % 16 + {0, 16, 32, 48}.
+__device__ __forceinline__ float max_xor16(float v)
+{
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     return fmaxf(__builtin_bit_cast(float, (uint32_t)p[0]), __builtin_bit_cast(float, (uint32_t)p[1]));
 }
 
@@ -125,6 +144,13 @@ __device__ __forceinline__ int wave_max(int v)
     return __builtin_amdgcn_readfirstlane(v);
 }
 
+__device__ __forceinline__ float max_wave(float v)
+{
+    #pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
+    return v;
+}
+
 // The key tiles (KT keys from dom_lo on) that some row with a position in [pmin, pmax] sees: `ns` tiles of
 // sinks, then the tiles from wt on; and the part [it0, it1) of that list that a split takes.
 struct TileList
@@ -171,14 +197,15 @@ struct Acc
     }
 };
 
-template <class IO, int HD>
-__device__ __forceinline__ void load_q(const AttnArgs& a, const QRow& r, int half, u32x4 (&qf)[HD / 16])
+// A row's B operand for steps of DK dimensions: part `part` of each step's 8-element parts.
+template <class IO, int HD, int DK>
+__device__ __forceinline__ void load_q(const AttnArgs& a, const QRow& r, int part, u32x4 (&qf)[HD / DK])
 {
     const uint16_t* src = (const uint16_t*)a.q + r.tok * a.q_ts + (int64_t)r.h * a.q_hs;
     #pragma unroll
-    for (int t = 0; t < HD / 16; ++t)
+    for (int t = 0; t < HD / DK; ++t)
     {
-        const int e = 16 * t + 8 * half;
+        const int e = DK * t + 8 * part;
         if (a.q_vec) qf[t] = *(gcptr<u32x4>)(src + e);
         else
         {
@@ -186,6 +213,20 @@ __device__ __forceinline__ void load_q(const AttnArgs& a, const QRow& r, int hal
             for (int i = 0; i < 4; ++i)
                 qf[t][i] = (uint32_t)((gcptr<uint16_t>)src)[e + 2 * i] | (uint32_t)((gcptr<uint16_t>)src)[e + 2 * i + 1] << 16;
         }
+    }
+}
+
+// Four elements of an output row.
+template <class IO>
+__device__ __forceinline__ void store_out4(const AttnArgs& a, int64_t tok, int h, int d, float x, float y, float z, float w)
+{
+    const gptr<uint16_t> p = (gptr<uint16_t>)((uint16_t*)a.out + tok * a.o_ts + (int64_t)h * a.o_hs + d);
+    const u32x2 v = { pack2<IO>(x, y), pack2<IO>(z, w) };
+    if (a.o_vec) *(gptr<u32x2>)p = v;
+    else
+    {
+        p[0] = (uint16_t)v.x; p[1] = (uint16_t)(v.x >> 16);
+        p[2] = (uint16_t)v.y; p[3] = (uint16_t)(v.y >> 16);
     }
 }
 
@@ -261,12 +302,42 @@ __device__ __forceinline__ bool nonfinite8(const u32x4& v)
     return c != 0;
 }
 
+// Zeroes the infinities and NaNs of v and returns their indicators: 1 for +inf, 64 for -inf, 65 for a NaN.
+template <class IO>
+__device__ __forceinline__ u32x4 take_nonfinite(u32x4& v)
+{
+    constexpr uint32_t E = IO::code == DT_F16 ? 0x7c00u : 0x7f80u;
+    u32x4 ind;
+    #pragma unroll
+    for (int e = 0; e < 4; ++e)
+    {
+        float w[2];
+        uint32_t keep = 0;
+        #pragma unroll
+        for (int k = 0; k < 2; ++k)
+        {
+            const uint32_t h = ((uint32_t)v[e] >> (16 * k)) & 0xffffu, mag = h & 0x7fffu;
+            w[k] = mag > E ? 65.0f : mag < E ? 0.0f : h >> 15 ? 64.0f : 1.0f;
+            keep |= mag < E ? 0xffffu << (16 * k) : 0u;
+        }
+        ind[e] = pack2<IO>(w[0], w[1]);
+        v[e] &= keep;
+    }
+    return ind;
+}
+// What n = (count of +inf) + 64 (count of -inf), NaNs in both, adds to a sum.
+__device__ __forceinline__ float nonfinite_sum(float n)
+{
+    const int c = (int)n;
+    return (c & 63 ? INFINITY : 0.0f) - (c >> 6 ? INFINITY : 0.0f);
+}
+
 // o^T += V^T P^T over 32 keys (LDS rows from vb on).  The probabilities are rounded to V's type for the matrix
 // cores: one rounding of at most half a step each, against the same maximum for the whole row; l sums them
 // unrounded.  CARE: V has infinities or NaNs and some row does not see some of these keys; there the probability
 // is 0, but 0 * inf and 0 * NaN must not reach the row.  They are then taken out of the product and applied by a
 // second one, of 1 where V has +inf or NaN, 64 where it has -inf or NaN and 65 for a NaN, with "the row's probability
-// is not 0": its sums over 16 keys tell how many of each a row sees.
+// is not 0": its sums over at most 32 keys tell how many of each a row sees.
 template <class IO, int HD, bool CARE>
 __device__ __forceinline__ void pv_tile(Acc<HD>& a, const f32x16& p, const char* vb, int lane)
 {
@@ -295,31 +366,11 @@ __device__ __forceinline__ void pv_tile(Acc<HD>& a, const f32x16& p, const char*
             u32x4 vf = { w0.x, w0.y, w1.x, w1.y };
             if constexpr (CARE)
             {
-                constexpr uint32_t E = IO::code == DT_F16 ? 0x7c00u : 0x7f80u;
-                u32x4 ind;
-                #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                {
-                    float w[2];
-                    uint32_t keep = 0;
-                    #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                    {
-                        const uint32_t h = ((uint32_t)vf[e] >> (16 * k)) & 0xffffu, mag = h & 0x7fffu;
-                        w[k] = mag > E ? 65.0f : mag < E ? 0.0f : h >> 15 ? 64.0f : 1.0f;
-                        keep |= mag < E ? 0xffffu << (16 * k) : 0u;
-                    }
-                    ind[e] = pack2<IO>(w[0], w[1]);
-                    vf[e] &= keep;
-                }
+                const u32x4 ind = take_nonfinite<IO>(vf);
                 f32x16 n{};
                 n = mfma32<IO>(ind, see, n);
                 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                {
-                    const int c = (int)n[i];
-                    a.o[t][i] += (c & 63 ? INFINITY : 0.0f) - (c >> 6 ? INFINITY : 0.0f);
-                }
+                for (int i = 0; i < 16; ++i) a.o[t][i] += nonfinite_sum(n[i]);
             }
             a.o[t] = mfma32<IO>(vf, pf, a.o[t]);
         }
@@ -418,7 +469,7 @@ __global__ __launch_bounds__(256, HD == 256 || NQ == 2 ? 1 : 2) void k_attn_rows
     for (int n = 0; n < NQ; ++n)
     {
         row[n] = query_row(a, it.set, it.kvh, min(r0 + 32 * n + (lane & 31), a.rows - 1));
-        load_q<IO, HD>(a, row[n], half, qf[n]);
+        load_q<IO, HD, 16>(a, row[n], half, qf[n]);
         acc[n].clear();
         pmin[n] = wave_min(row[n].p);
         pmax[n] = wave_max(row[n].p);
@@ -513,26 +564,16 @@ __global__ __launch_bounds__(256, HD == 256 || NQ == 2 ? 1 : 2) void k_attn_rows
         {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             if (a.lse && half == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (fmaf(acc[n].m, a.c, -kShift<IO>) + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f;
-            uint16_t* dst = (uint16_t*)a.out + row[n].tok * a.o_ts + (int64_t)row[n].h * a.o_hs + 4 * half;
             #pragma unroll
             for (int t = 0; t < HD / 32; ++t)
                 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                {
-                    const u32x2 w = { pack2<IO>(acc[n].o[t][4 * g] * inv, acc[n].o[t][4 * g + 1] * inv),
-                                      pack2<IO>(acc[n].o[t][4 * g + 2] * inv, acc[n].o[t][4 * g + 3] * inv) };
-                    gptr<uint16_t> d = (gptr<uint16_t>)(dst + 32 * t + 8 * g);
-                    if (a.o_vec) *(gptr<u32x2>)d = w;
-                    else
-                    {
-                        d[0] = (uint16_t)w.x; d[1] = (uint16_t)(w.x >> 16);
-                        d[2] = (uint16_t)w.y; d[3] = (uint16_t)(w.y >> 16);
-                    }
-                }
+                    store_out4<IO>(a, row[n].tok, row[n].h, 32 * t + 8 * g + 4 * half, acc[n].o[t][4 * g] * inv,
+                                   acc[n].o[t][4 * g + 1] * inv, acc[n].o[t][4 * g + 2] * inv, acc[n].o[t][4 * g + 3] * inv);
         }
         else
         {
-            const int64_t pr = (int64_t)(a.split0 + it.split) * a.rows_all + gr;
+            const int64_t pr = gr * a.splits + a.split0 + it.split;
             if (half == 0) { a.pml[2 * pr] = fmaf(acc[n].m, a.c, -kShift<IO>); a.pml[2 * pr + 1] = l; }
             if (l == 0.0f) continue;
             gptr<f32x4> d = (gptr<f32x4>)(a.po + pr * HD + 4 * half);
@@ -546,29 +587,37 @@ __global__ __launch_bounds__(256, HD == 256 || NQ == 2 ? 1 : 2) void k_attn_rows
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few query rows (decode): the 4 waves of a workgroup hold the same 32 rows and walk different tiles of 32 keys,
-// each through its own part of LDS without a barrier; their results are joined at the end.
-template <class IO, int HD, bool SMALL>
+// Few query rows (decode): the 4 waves of a workgroup hold the same NC * 16 rows and walk different tiles of 32 keys,
+// each through its own part of LDS without a barrier; their results are joined at the end.  With 16 rows per MFMA
+// column tile (v_mfma_f32_16x16x32: lane l holds row l % 16, keys 4 (l / 16) + i of each 16) a group of 8 or 16 query
+// heads leaves little of a tile empty, and o, Q and the scores take half the registers of 32 rows, so that two tiles
+// of loads per SIMD stay in flight: HBM is the bound here.
+template <class IO, int HD, int NC, bool SMALL>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a)
 {
-    constexpr int KT = 32, CH = HD / 8, RB = HD * 2, STEPS = KT * CH / 64;
+    constexpr int KT = 32, CH = HD / 8, RB = HD * 2, STEPS = KT * CH / 64, ROWS = 16 * NC;
     __shared__ __align__(16) char lds[4][2 * KT * RB];
-    __shared__ float mlw[4][2][32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    __shared__ float mlw[4][2][ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, col = lane & 15;
     char* const kl = lds[wave];
     char* const vl = lds[wave] + KT * RB;
     const Item it = launch_item(a);
-    const int r0 = it.tile * 32;
-    const QRow row = query_row(a, it.set, it.kvh, min(r0 + (lane & 31), a.rows - 1));
-    if (it.split == 0 && it.kvh == 0) flag_positions(a, row);
-    const int pmin = wave_min(row.p), pmax = wave_max(row.p);
+    const int r0 = it.tile * ROWS;
+    QRow row[NC];
+    int pmin = 0x7fffffff, pmax = -0x7fffffff;
+    #pragma unroll
+    for (int n = 0; n < NC; ++n)
+    {
+        row[n] = query_row(a, it.set, it.kvh, min(r0 + 16 * n + col, a.rows - 1));
+        if (it.split == 0 && it.kvh == 0) flag_positions(a, row[n]);
+        pmin = min(pmin, row[n].p);
+        pmax = max(pmax, row[n].p);
+    }
+    pmin = wave_min(pmin);
+    pmax = wave_max(pmax);
     const TileList tl = tile_list(a, pmin, pmax, KT);
     const int per = ((tl.count + a.nsplit - 1) / a.nsplit + 3) & ~3;
     const int t0 = min(it.split * per, tl.count), t1 = min(t0 + per, tl.count);
-    u32x4 qf[HD / 16];
-    Acc<HD> acc;
-    acc.clear();
-    load_q<IO, HD>(a, row, half, qf);
 
     const int32_t* table = a.table + (a.whole ? 0 : (int64_t)it.set * a.max_blocks);
     u32x4 ks[STEPS], vs[STEPS];
@@ -586,6 +635,25 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
     };
     fetch_entry(t0 + wave);
     if (t0 + wave < t1) { stage(t0 + wave); fetch_entry(t0 + wave + 4); }
+
+    u32x4 qf[NC][HD / 32];
+    f32x4 o[NC][HD / 16];
+    float m[NC], l[NC];
+    #pragma unroll
+    for (int n = 0; n < NC; ++n)
+    {
+        load_q<IO, HD, 32>(a, row[n], quad, qf[n]);
+        #pragma unroll
+        for (int t = 0; t < HD / 16; ++t) o[n][t] = f32x4{};
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+    }
+    // K fragment: key row col (of 16), chunks 4 t + quad; V^T fragment: keys 4 quad + 0..3 (and + 16), columns 16 t + col
+    const char* const krow = kl + col * RB;
+    const int kx = (swz<HD>(col) ^ quad) << 4;
+    const int vkey = 4 * quad + (col >> 2);
+    const char* const vrow = vl + vkey * RB + ((col & 1) << 3);
+    const int vx = (swz<HD>(vkey) ^ ((col >> 1) & 1)) << 4;
     for (int i = t0 + wave; i < t1; i += 4)
     {
         const uint32_t ok = ok_next;
@@ -614,114 +682,209 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         wave_lds_fence();
         if (i + 4 < t1) { stage(i + 4); fetch_entry(i + 8); }
         if (ok == 0) continue;
-        f32x16 s = qk_tile<IO, HD>(kl, lane, qf);
-        if (!whole) mask_tile(s, j, half, row.p, a.window, a.sinks, ok);
-        softmax_tile<IO, HD>(acc, s, a.c);
-        if (!care) pv_tile<IO, HD, false>(acc, s, vl, lane);
-        else pv_tile<IO, HD, true>(acc, s, vl, lane);
+        f32x4 s[NC][2];
+        #pragma unroll
+        for (int k = 0; k < 2; ++k)
+        {
+            #pragma unroll
+            for (int n = 0; n < NC; ++n) s[n][k] = f32x4{};
+            #pragma unroll
+            for (int t = 0; t < HD / 32; ++t)
+            {
+                const u32x4 kf = *(const u32x4*)(krow + k * 16 * RB + (kx ^ (t << 6)));
+                #pragma unroll
+                for (int n = 0; n < NC; ++n) s[n][k] = mfma16<IO>(kf, qf[n][t], s[n][k]);
+            }
+        }
+        u32x4 pf[NC], see[NC];
+        #pragma unroll
+        for (int n = 0; n < NC; ++n)
+        {
+            if (!whole)
+            {
+                const int p = row[n].p, lo = a.window > 0 ? p - a.window + 1 : 0;
+                const uint32_t okq = ok >> (4 * quad);
+                #pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        const int jj = j + 4 * quad + 16 * k + e;
+                        const bool vis = (jj <= p) & ((jj >= lo) | (jj < a.sinks)) & (((okq >> (16 * k + e)) & 1u) != 0);
+                        s[n][k][e] = vis ? s[n][k][e] : -INFINITY;
+                    }
+            }
+            float mx = s[n][0][0];
+            #pragma unroll
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[n][e >> 2][e & 3]);
+            const float mn = fmaxf(m[n], max_xor32(max_xor16(mx)));
+            const float ref = (mn == -INFINITY ? 0.0f : mn) * a.c;
+            const float alpha = __builtin_amdgcn_exp2f(fmaf(m[n], a.c, -ref));
+            float sum = 0.0f, pr[8];
+            #pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                pr[e] = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], a.c, kShift<IO> - ref));
+                sum += pr[e];
+            }
+            l[n] = fmaf(l[n], alpha, sum);
+            m[n] = mn;
+            #pragma unroll
+            for (int e = 0; e < 4; ++e)
+            {
+                pf[n][e] = pack2<IO>(pr[2 * e], pr[2 * e + 1]);
+                see[n][e] = pack2<IO>(pr[2 * e] != 0.0f ? 1.0f : 0.0f, pr[2 * e + 1] != 0.0f ? 1.0f : 0.0f);
+            }
+            #pragma unroll
+            for (int t = 0; t < HD / 16; ++t)
+                #pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][t][e] *= alpha;
+        }
+        #pragma unroll
+        for (int t = 0; t < HD / 16; ++t)
+        {
+            const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(vrow + (vx ^ (t << 5))));
+            const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(vrow + 16 * RB + (vx ^ (t << 5))));
+            const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+            u32x4 vf = { w0.x, w0.y, w1.x, w1.y };
+            if (care)
+            {
+                const u32x4 ind = take_nonfinite<IO>(vf);
+                #pragma unroll
+                for (int n = 0; n < NC; ++n)
+                {
+                    const f32x4 c = mfma16<IO>(ind, see[n], f32x4{});
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][t][e] += nonfinite_sum(c[e]);
+                }
+            }
+            #pragma unroll
+            for (int n = 0; n < NC; ++n) o[n][t] = mfma16<IO>(vf, pf[n], o[n][t]);
+        }
     }
     // Join the waves: o against the common maximum, through LDS as [row][HD] floats with the 16-byte chunks of a
     // row permuted by its low bits.
-    const float lw = sum_xor32(acc.l);
-    if (half == 0) { mlw[wave][0][lane] = acc.m; mlw[wave][1][lane] = lw; }
-    wave_lds_fence();
-    const int rl = lane & 31;
+    float lw[NC];
+    #pragma unroll
+    for (int n = 0; n < NC; ++n)
+    {
+        lw[n] = sum_xor32(sum_xor16(l[n]));
+        if (quad == 0) { mlw[wave][0][16 * n + col] = m[n]; mlw[wave][1][16 * n + col] = lw[n]; }
+    }
     __syncthreads();
-    float m = -INFINITY;
     #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, mlw[w][0][rl]);
-    const float ref = (m == -INFINITY ? 0.0f : m) * a.c;
-    const float f = __builtin_amdgcn_exp2f(fmaf(acc.m, a.c, -ref));
-    const bool some = lw != 0.0f;
-    #pragma unroll
-    for (int t = 0; t < HD / 32; ++t)
+    for (int n = 0; n < NC; ++n)
+    {
+        const int r = 16 * n + col;
+        float mm = -INFINITY;
         #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mlw[w][0][r]);
+        const float ref = (mm == -INFINITY ? 0.0f : mm) * a.c;
+        const float f = __builtin_amdgcn_exp2f(fmaf(m[n], a.c, -ref));
+        #pragma unroll
+        for (int t = 0; t < HD / 16; ++t)
         {
-            const int ch = (8 * t + 2 * g + half) ^ (rl & 7);
             f32x4 w;
             #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = some ? acc.o[t][4 * g + e] * f : 0.0f;
-            *(f32x4*)(kl + rl * (HD * 4) + ch * 16) = w;
+            for (int e = 0; e < 4; ++e) w[e] = lw[n] != 0.0f ? o[n][t][e] * f : 0.0f;
+            *(f32x4*)(kl + r * (HD * 4) + (((4 * t + quad) ^ (col & 7)) << 4)) = w;
         }
+    }
     __syncthreads();
     // 256 lanes walk the rows: HD / 4 lanes of four columns each per row.
     constexpr int LPR = HD / 4, RPS = 256 / LPR;
-    const int nr = min(32, a.rows - r0);
+    const int nr = min(ROWS, a.rows - r0);
     for (int r = tid / LPR; r < nr; r += RPS)
     {
         const int ch = tid % LPR;
-        f32x4 o{};
-        float mm = -INFINITY, l = 0.0f;
+        f32x4 sum{};
+        float mm = -INFINITY, ls = 0.0f;
         #pragma unroll
         for (int w = 0; w < 4; ++w)
         {
-            o += *(const f32x4*)(lds[w] + r * (HD * 4) + ((ch ^ (r & 7)) << 4));
+            const f32x4 v = *(const f32x4*)(lds[w] + r * (HD * 4) + ((ch ^ (r & 7)) << 4));
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += v[e];
             mm = fmaxf(mm, mlw[w][0][r]);
         }
         const float rf = (mm == -INFINITY ? 0.0f : mm) * a.c;
         #pragma unroll
-        for (int w = 0; w < 4; ++w) l = fmaf(mlw[w][1][r], __builtin_amdgcn_exp2f(fmaf(mlw[w][0][r], a.c, -rf)), l);
+        for (int w = 0; w < 4; ++w) ls = fmaf(mlw[w][1][r], __builtin_amdgcn_exp2f(fmaf(mlw[w][0][r], a.c, -rf)), ls);
         const QRow qr = query_row(a, it.set, it.kvh, r0 + r);
         const int64_t gr = qr.tok * a.hq + qr.h;
         if (a.direct)
         {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (a.lse && ch == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (rf - kShift<IO> + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f;
-            gptr<uint16_t> d = (gptr<uint16_t>)((uint16_t*)a.out + qr.tok * a.o_ts + (int64_t)qr.h * a.o_hs + 4 * ch);
-            const u32x2 w = { pack2<IO>(o.x * inv, o.y * inv), pack2<IO>(o.z * inv, o.w * inv) };
-            if (a.o_vec) *(gptr<u32x2>)d = w;
-            else
-            {
-                d[0] = (uint16_t)w.x; d[1] = (uint16_t)(w.x >> 16);
-                d[2] = (uint16_t)w.y; d[3] = (uint16_t)(w.y >> 16);
-            }
+            const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+            if (a.lse && ch == 0) a.lse[gr] = ls == 0.0f ? -INFINITY : (rf - kShift<IO> + __builtin_amdgcn_logf(ls)) * 0.69314718055994530942f;
+            store_out4<IO>(a, qr.tok, qr.h, 4 * ch, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
         }
         else
         {
-            const int64_t pr = (int64_t)(a.split0 + it.split) * a.rows_all + gr;
-            if (ch == 0) { a.pml[2 * pr] = fmaf(mm, a.c, -kShift<IO>); a.pml[2 * pr + 1] = l; }
-            if (l != 0.0f) ((gptr<f32x4>)(a.po + pr * HD))[ch] = o;
+            const int64_t pr = gr * a.splits + a.split0 + it.split;
+            if (ch == 0) { a.pml[2 * pr] = fmaf(mm, a.c, -kShift<IO>); a.pml[2 * pr + 1] = ls; }
+            if (ls != 0.0f) ((gptr<f32x4>)(a.po + pr * HD))[ch] = sum;
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the splits of a row: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  A wave per row.
-template <class IO, int HD>
+// Joins the splits of a row: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  WAVES waves per row; a wave takes
+// 256 / HD splits at a time (HD / 4 lanes of four columns each).
+template <class IO, int HD, int WAVES>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a)
 {
-    const int64_t gr = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (gr >= a.rows_all) return;
-    const int lane = threadIdx.x & 63, ns = a.nsplit;
-    float m = -INFINITY;
+    constexpr int LPR = HD / 4, SPW = 64 / LPR;       // lanes per partial row, partial rows per wave
+    __shared__ float wt[4 / WAVES][kMaxSplits];
+    __shared__ f32x4 part[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, local = wave / WAVES, sub = wave % WAVES;
+    const int64_t gr = min((int64_t)blockIdx.x * (4 / WAVES) + local, a.rows_all - 1);
+    const int ns = a.splits;
+    const gcptr<f32x2> ml = (gcptr<f32x2>)(a.pml + 2 * gr * ns);
+    float m = -INFINITY, l = 0.0f;
     for (int i = lane; i < ns; i += 64)
     {
-        const float* e = a.pml + 2 * ((int64_t)i * a.rows_all + gr);
-        if (e[1] != 0.0f) m = fmaxf(m, e[0]);
+        const f32x2 e = ml[i];
+        if (e.y != 0.0f) m = fmaxf(m, e.x);
     }
-    #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    constexpr int E = HD / 64;
-    float o[E] = {}, l = 0.0f;
-    for (int i = 0; i < ns; ++i)
+    m = max_wave(m);
+    for (int i = lane; i < ns; i += 64)
     {
-        const float* e = a.pml + 2 * ((int64_t)i * a.rows_all + gr);
-        const float li = e[1];
-        if (li == 0.0f) continue;
-        const float w = __builtin_amdgcn_exp2f(e[0] - (m == -INFINITY ? 0.0f : m));
-        l = fmaf(w, li, l);
-        const float* p = a.po + ((int64_t)i * a.rows_all + gr) * HD + lane * E;
-        #pragma unroll
-        for (int k = 0; k < E; ++k) o[k] = fmaf(w, p[k], o[k]);
+        const f32x2 e = ml[i];
+        const float w = e.y != 0.0f ? __builtin_amdgcn_exp2f(e.x - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+        if (sub == 0) wt[local][i] = e.y != 0.0f ? w : -1.0f;      // -1: nothing was written
+        if (e.y != 0.0f) l = fmaf(w, e.y, l);
     }
+    l = group_sum<64>(l);
+    __syncthreads();
+    f32x4 o{};
+    const gcptr<f32x4> po = (gcptr<f32x4>)(a.po + gr * ns * HD) + lane % LPR;
+    #pragma unroll 4
+    for (int i = sub * SPW + lane / LPR; i < ns; i += WAVES * SPW)
+    {
+        const float w = wt[local][i];
+        if (w < 0.0f) continue;
+        const f32x4 p = po[(int64_t)i * LPR];
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(w, p[e], o[e]);
+    }
+    part[wave][lane] = o;
+    __syncthreads();
+    if (sub != 0 || lane >= LPR || (int64_t)blockIdx.x * (4 / WAVES) + local >= a.rows_all) return;
+    #pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+        #pragma unroll
+        for (int k = 0; k < SPW; ++k)
+        {
+            if (w == 0 && k == 0) continue;
+            const f32x4 p = part[local * WAVES + w][k * LPR + lane];
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += p[e];
+        }
     const int64_t tok = gr / a.hq;
     const int h = (int)(gr - tok * a.hq);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (a.lse && lane == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f;
-    uint16_t* d = (uint16_t*)a.out + tok * a.o_ts + (int64_t)h * a.o_hs + lane * E;
-    #pragma unroll
-    for (int k = 0; k < E; ++k) ((gptr<uint16_t>)d)[k] = (uint16_t)pack2<IO>(o[k] * inv, 0.0f);
+    store_out4<IO>(a, tok, h, 4 * lane, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 }  // namespace exl3r
@@ -732,7 +895,7 @@ namespace {
 
 struct Phase
 {
-    bool rows_kernel;
+    int cols;       // 0: k_attn_rows; 1, 2: k_attn_keys with that many column tiles
     int64_t sets, rows, row_tiles, nsplit;
 };
 
@@ -740,15 +903,17 @@ struct Phase
 Phase plan_phase(int64_t sets, int64_t rows, int hk, int64_t span)
 {
     Phase p;
-    p.rows_kernel = rows > 64;
+    p.cols = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
     p.sets = sets;
     p.rows = rows;
-    p.row_tiles = (rows + (p.rows_kernel ? 127 : 31)) / (p.rows_kernel ? 128 : 32);
+    const int64_t per_tile = p.cols ? 16 * p.cols : 128;
+    p.row_tiles = (rows + per_tile - 1) / per_tile;
     const int64_t base = sets * hk * p.row_tiles;
-    const int64_t want = p.rows_kernel ? 512 : 1024, least = p.rows_kernel ? 256 : 128;
+    const int64_t want = p.cols ? 4096 : 512, least = p.cols ? 128 : 256;
     int64_t n = (want + base - 1) / base;
     const int64_t most = (span + least - 1) / least;
     if (n > most) n = most;
+    if (n > kMaxSplits / 2) n = kMaxSplits / 2;
     p.nsplit = n < 1 ? 1 : n;
     return p;
 }
@@ -811,7 +976,8 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
     if ((hq > 1 && (q_hs < hd || o_hs < hd)) || (tokens > 1 && (q_ts < hd || o_ts < hd)))
         return set_error(EXL3R_EINVAL, "%s: strides shorter than a head", op);
     const Plan p = make_plan(bsz, seq, hq, hk, hd, cap, window, sinks, shared);
-    if (p.own.sets * hk * p.own.row_tiles * p.own.nsplit > 0xffffff || p.prefix.sets * hk * p.prefix.row_tiles * p.prefix.nsplit > 0xffffff)
+    if (p.own.sets * hk * p.own.row_tiles * p.own.nsplit > 0xffffff || p.prefix.sets * hk * p.prefix.row_tiles * p.prefix.nsplit > 0xffffff ||
+        (p.join && tokens * hq > 0xffffff))
         return set_error(EXL3R_EINVAL, "%s: more than 2^24 workgroups", op);
     if (p.join && (!ws || ((uintptr_t)ws & 255) || ws_bytes < p.bytes))
         return set_error(EXL3R_EINVAL, "%s: the workspace must be 256-byte aligned and hold %zu bytes (%zu given)", op, p.bytes, ws ? ws_bytes : 0);
@@ -827,6 +993,7 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
     a.err = err;
     a.rows_all = tokens * hq;
     a.po = (float*)ws;
+    a.splits = (int)p.splits;
     a.pml = p.join ? (float*)ws + p.splits * a.rows_all * hd : nullptr;
     a.q_ts = q_ts; a.q_hs = q_hs; a.o_ts = o_ts; a.o_hs = o_hs;
     a.max_blocks = max_blocks;
@@ -854,24 +1021,28 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
             x.nsplit = (int)ph.nsplit;
             x.split0 = (int)split0;
             const int64_t grid = ph.sets * hk * ph.row_tiles * ph.nsplit;
-            if (ph.rows_kernel)
+            if (ph.cols == 0)
             {
                 if (page_size < 64) launch(k_attn_rows<IO, HD, 1, true>, (unsigned)grid, 256, 0, st, x);
                 else launch(k_attn_rows<IO, HD, 1, false>, (unsigned)grid, 256, 0, st, x);
             }
+            else if (ph.cols == 1)
+            {
+                if (page_size < 32) launch(k_attn_keys<IO, HD, 1, true>, (unsigned)grid, 256, 0, st, x);
+                else launch(k_attn_keys<IO, HD, 1, false>, (unsigned)grid, 256, 0, st, x);
+            }
             else
             {
-                if (page_size < 32) launch(k_attn_keys<IO, HD, true>, (unsigned)grid, 256, 0, st, x);
-                else launch(k_attn_keys<IO, HD, false>, (unsigned)grid, 256, 0, st, x);
+                if (page_size < 32) launch(k_attn_keys<IO, HD, 2, true>, (unsigned)grid, 256, 0, st, x);
+                else launch(k_attn_keys<IO, HD, 2, false>, (unsigned)grid, 256, 0, st, x);
             }
         };
         if (shared > 0) phase(p.prefix, true, 0, shared, 0);
         phase(p.own, false, shared, cap, p.prefix.nsplit);
         if (p.join)
         {
-            AttnArgs x = a;
-            x.nsplit = (int)p.splits;
-            launch(k_attn_join<IO, HD>, (unsigned)((a.rows_all + 3) / 4), 256, 0, st, x);
+            if (p.splits > 16) launch(k_attn_join<IO, HD, 4>, (unsigned)a.rows_all, 256, 0, st, a);
+            else launch(k_attn_join<IO, HD, 1>, (unsigned)((a.rows_all + 3) / 4), 256, 0, st, a);
         }
     };
     auto by_dim = [&](auto T) {

@@ -372,6 +372,27 @@ __device__ __forceinline__ float round1(float v, int dt)
     return v;
 }
 
+// A whole chunk of 8 logits.  ALIGNED: 16-byte aligned rows; otherwise (an odd vocabulary, a sliced tensor)
+// the same 16-byte accesses at the alignment of one element, which the hardware splits where they cross a
+// line, in place of 8 single reads and, for a draw, 8 Philox blocks instead of 2 (64 x 151935 f32 logits, us,
+// before and after: argmax 24.6 -> 13.6, draw 34.8 -> 15.4).
+typedef u32x4 __attribute__((aligned(2))) u32x4_u2;
+typedef u32x4 __attribute__((aligned(4))) u32x4_u4;
+template <class IT, bool ALIGNED>
+__device__ __forceinline__ typename IT::Vec load_chunk(const void* base, int64_t c)
+{
+    if constexpr (ALIGNED) return load8s<IT>(base, c);
+    else if constexpr (IT::code == DT_F32)
+    {
+        const gcptr<u32x4_u4> p = (gcptr<u32x4_u4>)((const float*)base + c);
+        typename IT::Vec v;
+        v.a = __builtin_nontemporal_load(p);
+        v.b = __builtin_nontemporal_load(p + 1);
+        return v;
+    }
+    else return { __builtin_nontemporal_load((gcptr<u32x4_u2>)((const uint16_t*)base + c)) };
+}
+
 // 8 elements of a runtime-typed vector (norm weights: tiny, L2-resident, uniform branch).
 __device__ __forceinline__ void load8_dyn(const void* base, int dt, int64_t e, float (&f)[8])
 {

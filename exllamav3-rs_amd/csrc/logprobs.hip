@@ -2,18 +2,24 @@
 //
 // With m the row's maximum, l = sum_c e^(x_c - m) and t = sum_c e^(x_c - m) (x_c - m):
 //   ln P_c = x_c - m - ln l,    entropy = ln l - t / l   (two terms >= 0: nothing cancels).
-// A row is cut into slices of a workgroup each; a slice keeps its running m, l, t and the maximum of every group
-// of 64 columns.  A second kernel, a workgroup per row, joins the slices and finds the top columns: with (value, lower
-// column first) as the order, the k largest columns are in the k groups with the largest (maximum, lower group
-// first), since each of those k groups has a column that precedes all columns of any other group.  Only these
-// groups are read again.
+// Each lane keeps a running m, l, t over steps of 32 columns (4 chunks of 8, 2048 apart, so a wave's loads are whole
+// lines), and the maximum of each of its steps: a group of 32 columns.  The top columns are then found from the group
+// maxima alone.  A lane's best group maximum is one column's value, so with T the k-th largest of the lanes' best, k
+// columns reach T at least, and every column among the k largest does: only the groups whose maximum reaches T, a few
+// more than k, are read again, and their columns that reach T, as (value, lower column) keys, ranked by counting.
 #include "abi.hpp"
 #include "common.cuh"
 
 namespace exl3r {
 
-constexpr int kLpGroup = 64;      // columns per group
+constexpr int kLpLanes = 256;
+constexpr int kLpChunks = 4;                                 // chunks of 8 columns per lane and step
+constexpr int kLpStep = kLpLanes * 8 * kLpChunks;            // columns per step of a workgroup
 constexpr int kLpMaxTop = 32;
+constexpr int kLpList = 64;                                  // groups read again at most in the usual way
+// Columns ranked at most: in the careful way, those of fewer than kLpMaxTop groups and, of the columns that share the
+// floor's value, fewer than kLpMaxTop and one round of the search.
+constexpr int kLpCands = kLpMaxTop * 8 * kLpChunks + kLpMaxTop + kLpLanes;
 
 struct LpArgs
 {
@@ -45,40 +51,28 @@ __device__ __forceinline__ uint32_t lp_order(float v)
 __device__ __forceinline__ uint64_t lp_key(float v, uint32_t i) { return ((uint64_t)lp_order(v) << 32) | (0xfffffffeu - i); }
 __device__ __forceinline__ uint32_t lp_index(uint64_t k) { return 0xfffffffeu - (uint32_t)k; }
 
-__device__ __forceinline__ uint64_t lp_block_max(uint64_t v, uint64_t* lds)
-{
-    #pragma unroll
-    for (int d = 1; d < 64; d <<= 1)
-    {
-        const uint64_t o = __shfl_xor(v, d);
-        v = o > v ? o : v;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) v = lds[w] > v ? lds[w] : v;
-    return v;
-}
-
 struct LpSum
 {
     float m = -INFINITY, l = 0.0f, t = 0.0f;
 
     // A -inf logit adds nothing (its x - m is kept finite for the product with its zero weight); a NaN or +inf
-    // makes l NaN.
-    __device__ __forceinline__ void add8(const float (&x)[8], float cm)
+    // makes l NaN.  cm: the maximum of x, NaNs aside.
+    template <int N>
+    __device__ __forceinline__ void add(const float (&x)[N], float cm)
     {
         const float mn = fmaxf(m, cm), ref = mn == -INFINITY ? 0.0f : mn;
         const float d = fmaxf(m - ref, -1e30f), r = __builtin_amdgcn_exp2f(d * kLog2e);
-        t = r * fmaf(d, l, t);
-        l *= r;
+        // four short sums, so that the long ones take one addition per step
+        float ls[4] = {}, ts[4] = {};
         #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < N; ++j)
         {
             const float u = x[j] - ref, e = __builtin_amdgcn_exp2f(u * kLog2e);
-            l += e;
-            t = fmaf(e, fmaxf(u, -1e30f), t);
+            ls[j & 3] += e;
+            ts[j & 3] = fmaf(e, fmaxf(u, -1e30f), ts[j & 3]);
         }
+        t = fmaf(r, fmaf(d, l, t), (ts[0] + ts[1]) + (ts[2] + ts[3]));
+        l = fmaf(r, l, (ls[0] + ls[1]) + (ls[2] + ls[3]));
         m = mn;
     }
     __device__ __forceinline__ void join(float m2, float l2, float t2)
@@ -92,119 +86,301 @@ struct LpSum
     }
 };
 
-// 256 lanes, 8 columns per lane and step: a group of 64 columns is 8 lanes of one step.
-template <class IT>
-__global__ __launch_bounds__(256) void k_lp_slices(LpArgs a, int64_t slice)
+// The columns of step `step`'s group of lane `tid`: chunk u starts at step * kLpStep + u * 2048 + 8 tid.
+__device__ __forceinline__ int64_t lp_column(int64_t group, int u)
 {
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x / (uint32_t)a.slices, sl = blockIdx.x % (uint32_t)a.slices;
-    const char* base = a.x + row * a.ld;
-    const int64_t end = min(a.n, (sl + 1) * slice);
-    LpSum s;
-    for (int64_t c = sl * slice + tid * 8; c < ((end + 63) & ~(int64_t)63); c += 2048)
+    return (group / kLpLanes) * kLpStep + u * (kLpLanes * 8) + (group % kLpLanes) * 8;
+}
+
+// One lane's part of step `step`: sums into s, returns the group's maximum (NaN if there is one).
+template <class IT, bool VEC>
+__device__ __forceinline__ float lp_step(const LpArgs& a, const char* base, int64_t step, int tid, LpSum& s)
+{
+    const int64_t g = step * kLpLanes + tid;
+    float x[8 * kLpChunks];
+    if (step * kLpStep + kLpStep <= a.n)
     {
-        float x[8];
+        typename IT::Vec v[kLpChunks];
         #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = c + j < end ? load1(base, IT::code, c + j) : -INFINITY;
-        float cm = x[0];
+        for (int u = 0; u < kLpChunks; ++u) v[u] = load_chunk<IT, VEC>(base, lp_column(g, u));
         #pragma unroll
-        for (int j = 1; j < 8; ++j) cm = lp_max_nan(cm, x[j]);
-        s.add8(x, cm != cm ? -INFINITY : cm);
-        float gm = cm;
-        #pragma unroll
-        for (int d = 1; d < 8; d <<= 1) gm = lp_max_nan(gm, __shfl_xor(gm, d));
-        if ((tid & 7) == 0 && a.top) a.gmax[row * a.groups + c / kLpGroup] = gm;
+        for (int u = 0; u < kLpChunks; ++u)
+        {
+            float f[8];
+            unpack8<IT>(v[u], f);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) x[8 * u + j] = f[j];
+        }
     }
+    else
+    {
+        #pragma unroll
+        for (int u = 0; u < kLpChunks; ++u)
+        {
+            const int64_t c = lp_column(g, u);
+            float f[8];
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = -INFINITY;
+            if (c + 8 <= a.n) unpack8<IT>(load_chunk<IT, VEC>(base, c), f);
+            else
+            {
+                #pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (c + j < a.n) f[j] = load1(base, IT::code, c + j);
+            }
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) x[8 * u + j] = f[j];
+        }
+    }
+    float gm = x[0];
+    #pragma unroll
+    for (int j = 1; j < 8 * kLpChunks; ++j) gm = lp_max_nan(gm, x[j]);
+    float cm = gm;
+    if (__any(gm != gm))
+    {
+        cm = x[0];
+        #pragma unroll
+        for (int j = 1; j < 8 * kLpChunks; ++j) cm = fmaxf(cm, x[j]);
+        cm = cm != cm ? -INFINITY : cm;
+    }
+    s.add(x, cm);
+    return gm;
+}
+
+// The workgroup's joined sums, in every lane (lds: 3 floats per wave).
+__device__ __forceinline__ LpSum lp_block_sum(LpSum s, float (*w)[3])
+{
     #pragma unroll
     for (int d = 1; d < 64; d <<= 1)
     {
         const float m2 = __shfl_xor(s.m, d), l2 = __shfl_xor(s.l, d), t2 = __shfl_xor(s.t, d);
         s.join(m2, l2, t2);
     }
-    __shared__ float w[4][3];
-    if ((tid & 63) == 0) { w[tid >> 6][0] = s.m; w[tid >> 6][1] = s.l; w[tid >> 6][2] = s.t; }
+    if ((threadIdx.x & 63) == 0) { w[threadIdx.x >> 6][0] = s.m; w[threadIdx.x >> 6][1] = s.l; w[threadIdx.x >> 6][2] = s.t; }
     __syncthreads();
-    if (tid == 0)
-    {
-        for (int i = 1; i < 4; ++i) s.join(w[i][0], w[i][1], w[i][2]);
-        float* p = a.part + 3 * (row * a.slices + sl);
-        p[0] = s.m; p[1] = s.l; p[2] = s.t;
-    }
+    s.m = w[0][0]; s.l = w[0][1]; s.t = w[0][2];
+    #pragma unroll
+    for (int i = 1; i < kLpLanes / 64; ++i) s.join(w[i][0], w[i][1], w[i][2]);
+    return s;
 }
 
-template <class IT>
-__global__ __launch_bounds__(256) void k_lp_rows(LpArgs a)
+struct LpShared
 {
-    __shared__ uint64_t red[4];
-    __shared__ uint32_t chosen[kLpMaxTop];
-    const int64_t row = blockIdx.x;
+    u32x4 best[kLpLanes / 4];
+    uint32_t list[kLpList];
+    uint64_t cand[kLpCands];
+    int nlist, nabove, ncand, nfound, count[2];
+    uint32_t floor;
+};
+
+// Everything a row's sums and group maxima give: m, l, t in every lane; `groups` maxima at gmax.
+template <class IT, class P>
+__device__ __forceinline__ void lp_finish(const LpArgs& a, int64_t row, float m, float l, float t, P gmax, int64_t groups,
+                                          LpShared& sh)
+{
     const int tid = threadIdx.x;
     const char* base = a.x + row * a.ld;
-    const float* part = a.part + 3 * row * a.slices;
-    float m = -INFINITY;
-    for (int i = 0; i < a.slices; ++i) m = fmaxf(m, part[3 * i]);
-    double l = 0.0, t = 0.0;
-    for (int i = 0; i < a.slices; ++i)
-    {
-        const float li = part[3 * i + 1];
-        if (li == 0.0f) continue;
-        const double d = (double)part[3 * i] - m, r = exp(d);
-        l += r * li;
-        t += r * (part[3 * i + 2] + d * li);
-    }
     // ln P = (x - m) - ln l: m + ln l would lose ln l beside a large m.  Nothing but -inf: no distribution.
-    const double ll = l == 0.0 ? (double)NAN : log(l);
-    const auto log_p = [&](int64_t c) { return (float)((double)load1(base, IT::code, c) - m - ll); };
-    if (tid == 0)
+    const double ll = l == 0.0f ? (double)NAN : log((double)l);
+    const auto log_p = [&](float x) { return (float)((double)x - m - ll); };
+    if (tid == kLpLanes - 64)
     {
         if (a.tokens)
         {
             const int64_t k = a.tokens[row];
             if (a.err && (k < 0 || k >= a.vocab)) *a.err = 1;
-            a.logprobs[row] = k < 0 || k >= a.n ? (ll != ll ? NAN : -INFINITY) : log_p(k);
+            a.logprobs[row] = k < 0 || k >= a.n ? (ll != ll ? NAN : -INFINITY) : log_p(load1(base, IT::code, k));
         }
-        if (a.entropy) a.entropy[row] = (float)(ll - t / l);
+        if (a.entropy) a.entropy[row] = (float)(ll - (double)t / l);
     }
-    const int top = a.top, ng = (int)min((int64_t)top, a.groups);
-    uint64_t last = ~0ull;
-    for (int i = 0; i < ng; ++i)
+    const int top = a.top;
+    if (!top) return;
+    // Eight of the lane's maxima at a time: one wait for their loads.
+    constexpr int B = 8;
+    uint32_t best = 0;
+    for (int64_t g0 = tid; g0 < groups; g0 += B * kLpLanes)
     {
-        uint64_t best = 0;
-        for (int64_t g = tid; g < a.groups; g += 256)
+        float v[B];
+        #pragma unroll
+        for (int i = 0; i < B; ++i) v[i] = g0 + i * kLpLanes < groups ? gmax[g0 + i * kLpLanes] : -INFINITY;
+        #pragma unroll
+        for (int i = 0; i < B; ++i)
         {
-            const uint64_t k = lp_key(a.gmax[row * a.groups + g], (uint32_t)g);
-            if (k < last && k > best) best = k;
+            const uint32_t k = lp_order(v[i]);
+            best = k > best ? k : best;
         }
-        last = lp_block_max(best, red);
-        if (tid == 0) chosen[i] = lp_index(last);
+    }
+    ((uint32_t*)sh.best)[tid] = best;
+    if (tid == 0) sh.nlist = sh.nabove = sh.ncand = sh.nfound = 0;
+    __syncthreads();
+    // The lane whose best has exactly top - 1 others before it (ties by lane) holds the floor.
+    int before = 0;
+    #pragma unroll 8
+    for (int i = 0; i < kLpLanes / 4; ++i)
+    {
+        const u32x4 o = sh.best[i];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) before += o[j] > best || (o[j] == best && 4 * i + j < tid);
+    }
+    if (before == top - 1) sh.floor = best;
+    __syncthreads();
+    uint32_t floor = sh.floor;
+    // (a lane without a group that reaches the floor has none to list)
+    for (int64_t g0 = tid; g0 < groups && best >= floor; g0 += B * kLpLanes)
+    {
+        float v[B];
+        #pragma unroll
+        for (int i = 0; i < B; ++i) v[i] = g0 + i * kLpLanes < groups ? gmax[g0 + i * kLpLanes] : -INFINITY;
+        #pragma unroll
+        for (int i = 0; i < B; ++i)
+        {
+            const int64_t g = g0 + i * kLpLanes;
+            const uint32_t k = lp_order(v[i]);
+            if (g < groups && k >= floor)
+            {
+                const int at = atomicAdd(&sh.nlist, 1);
+                if (at < kLpList) sh.list[at] = (uint32_t)g;
+                if (k > floor) atomicAdd(&sh.nabove, 1);
+            }
+        }
     }
     __syncthreads();
-    uint64_t keys[kLpMaxTop * kLpGroup / 256];
-    #pragma unroll
-    for (int i = 0; i < kLpMaxTop * kLpGroup / 256; ++i)
+    const int listed = sh.nlist, above = sh.nabove;
+    if (listed <= kLpList)
     {
-        const int at = i * 256 + tid;
-        keys[i] = 0;
-        if (at < ng * kLpGroup)
+        for (int i = tid; i < listed * kLpChunks * 8; i += kLpLanes)
         {
-            const int64_t c = (int64_t)chosen[at / kLpGroup] * kLpGroup + at % kLpGroup;
-            if (c < a.n) keys[i] = lp_key(load1(base, IT::code, c), (uint32_t)c);
+            const int64_t c = lp_column(sh.list[i / (kLpChunks * 8)], (i / 8) % kLpChunks) + i % 8;
+            const float x = c < a.n ? load1(base, IT::code, c) : 0.0f;
+            if (c < a.n && lp_order(x) >= floor)
+            {
+                const int at = atomicAdd(&sh.ncand, 1);
+                if (at < kLpCands) sh.cand[at] = lp_key(x, (uint32_t)c);
+            }
         }
     }
-    last = ~0ull;
-    for (int r = 0; r < top; ++r)
+    __syncthreads();
+    if (listed > kLpList || sh.ncand > kLpCands)
     {
-        uint64_t best = 0;
-        #pragma unroll
-        for (int i = 0; i < kLpMaxTop * kLpGroup / 256; ++i) best = keys[i] < last && keys[i] > best ? keys[i] : best;
-        last = lp_block_max(best, red);
-        if (tid == 0)
+        // The careful way: many columns share the floor's value (a masked or a constant row), or a few lanes hold many
+        // of the largest.  The floor becomes the top-th largest group maximum, unless fewer than top are above it as it is ...
+        if (above >= top)
         {
-            const int64_t c = lp_index(last);
-            a.top_ids[row * top + r] = c;
-            a.top_logprobs[row * top + r] = log_p(c);
+            uint32_t v = 0;
+            for (int b = 31; b >= 0; --b)
+            {
+                const uint32_t w = v | (1u << b);
+                int n = 0;
+                for (int64_t g = tid; g < groups; g += kLpLanes) n += lp_order(gmax[g]) >= w;
+                if (tid == 0) sh.count[b & 1] = 0;
+                __syncthreads();
+                atomicAdd(&sh.count[b & 1], n);
+                __syncthreads();
+                if (sh.count[b & 1] >= top) v = w;
+            }
+            floor = v;
+        }
+        __syncthreads();
+        if (tid == 0) sh.ncand = 0;
+        __syncthreads();
+        // ... the columns above it are in the fewer than top groups above it ...
+        for (int64_t g = tid; g < groups; g += kLpLanes)
+            if (lp_order(gmax[g]) > floor)
+                for (int u = 0; u < kLpChunks; ++u)
+                    for (int64_t c = lp_column(g, u), e = min(c + 8, a.n); c < e; ++c)
+                    {
+                        const float x = load1(base, IT::code, c);
+                        if (lp_order(x) > floor) sh.cand[atomicAdd(&sh.ncand, 1)] = lp_key(x, (uint32_t)c);
+                    }
+        __syncthreads();
+        // ... and the first columns that equal it follow.
+        for (int64_t c0 = 0; c0 < a.n; c0 += kLpLanes)
+        {
+            const int64_t c = c0 + tid;
+            const float x = c < a.n ? load1(base, IT::code, c) : 0.0f;
+            if (c < a.n && lp_order(x) == floor)
+            {
+                sh.cand[atomicAdd(&sh.ncand, 1)] = lp_key(x, (uint32_t)c);
+                atomicAdd(&sh.nfound, 1);
+            }
+            __syncthreads();
+            const bool done = sh.nfound >= top;
+            __syncthreads();
+            if (done) break;
         }
     }
+    const int n = sh.ncand;
+    for (int i = tid; i < n; i += kLpLanes)
+    {
+        const uint64_t k = sh.cand[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += sh.cand[j] > k;
+        if (rank < top)
+        {
+            const int64_t c = lp_index(k);
+            a.top_ids[row * top + rank] = c;
+            a.top_logprobs[row * top + rank] = log_p(load1(base, IT::code, c));
+        }
+    }
+}
+
+// Few rows: a workgroup per slice of a row (a.slices of them, of `steps` steps), sums and maxima to the workspace ...
+template <class IT, bool VEC>
+__global__ __launch_bounds__(kLpLanes) void k_lp_slices(LpArgs a, int steps)
+{
+    __shared__ float w[kLpLanes / 64][3];
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x / (uint32_t)a.slices, sl = blockIdx.x % (uint32_t)a.slices;
+    const char* base = a.x + row * a.ld;
+    LpSum s;
+    for (int64_t i = sl * steps; i < (sl + 1) * steps && i * kLpStep < a.n; ++i)
+    {
+        const float gm = lp_step<IT, VEC>(a, base, i, tid, s);
+        if (a.top) a.gmax[row * a.groups + i * kLpLanes + tid] = gm;
+    }
+    s = lp_block_sum(s, w);
+    if (tid == 0)
+    {
+        float* p = a.part + 3 * (row * a.slices + sl);
+        p[0] = s.m; p[1] = s.l; p[2] = s.t;
+    }
+}
+
+// ... and a workgroup per row over them.
+template <class IT>
+__global__ __launch_bounds__(kLpLanes) void k_lp_join(LpArgs a)
+{
+    __shared__ LpShared sh;
+    const int64_t row = blockIdx.x;
+    __shared__ float w[kLpLanes / 64][3];
+    LpSum s;
+    if ((int)threadIdx.x < a.slices)
+    {
+        const gcptr<float> p = (gcptr<float>)a.part + 3 * (row * a.slices + threadIdx.x);
+        s.m = p[0]; s.l = p[1]; s.t = p[2];
+    }
+    s = lp_block_sum(s, w);
+    lp_finish<IT>(a, row, s.m, s.l, s.t, (gcptr<float>)a.gmax + row * a.groups, a.groups, sh);
+}
+
+// Many rows: a workgroup per row, its group maxima in LDS.
+template <class IT, bool VEC>
+__global__ __launch_bounds__(kLpLanes) void k_lp_rows(LpArgs a)
+{
+    extern __shared__ float gmax[];
+    __shared__ LpShared sh;
+    __shared__ float w[kLpLanes / 64][3];
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const char* base = a.x + row * a.ld;
+    LpSum s;
+    for (int64_t i = 0; i * kLpStep < a.n; ++i)
+    {
+        const float gm = lp_step<IT, VEC>(a, base, i, tid, s);
+        if (a.top) gmax[i * kLpLanes + tid] = gm;
+    }
+    s = lp_block_sum(s, w);
+    lp_finish<IT>(a, row, s.m, s.l, s.t, gmax, a.groups, sh);
 }
 
 }  // namespace exl3r
@@ -215,19 +391,21 @@ namespace {
 
 struct LpPlan
 {
-    int64_t slice, slices, groups;
+    bool by_rows;
+    int64_t steps, slices, groups;      // steps per slice
     size_t part_bytes, bytes;
 };
 
-LpPlan lp_plan(int64_t rows, int64_t vocab)
+LpPlan lp_plan(int64_t rows, int64_t n)
 {
     LpPlan p;
-    p.slice = 8192;
-    while ((vocab + p.slice - 1) / p.slice > 256) p.slice *= 2;
-    p.slices = (vocab + p.slice - 1) / p.slice;
-    p.groups = (vocab + kLpGroup - 1) / kLpGroup;
+    const int64_t all = (n + kLpStep - 1) / kLpStep;
+    p.groups = all * kLpLanes;
+    p.by_rows = rows >= 512 && p.groups * 4 <= 64 << 10;
+    p.steps = (all + 255) / 256;
+    p.slices = (all + p.steps - 1) / p.steps;
     p.part_bytes = ((size_t)rows * p.slices * 12 + 255) & ~(size_t)255;
-    p.bytes = p.part_bytes + (((size_t)rows * p.groups * 4 + 255) & ~(size_t)255);
+    p.bytes = p.by_rows ? 0 : p.part_bytes + (size_t)rows * p.groups * 4;
     return p;
 }
 
@@ -259,7 +437,7 @@ extern "C" int exl3r_token_logprobs(const void* logits, int dtype, int64_t rows,
     if (!logits || (tokens && !logprobs) || (top_k && (!top_ids || !top_logprobs)))
         return set_error(EXL3R_EINVAL, "%s: logits and the outputs asked for must be non-null", op);
     const LpPlan p = lp_plan(rows, n);
-    if (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.bytes)
+    if (p.bytes && (!workspace || ((uintptr_t)workspace & 255) || workspace_bytes < p.bytes))
         return set_error(EXL3R_EINVAL, "%s: the workspace must be 256-byte aligned and hold %zu bytes (%zu given)", op, p.bytes,
                          workspace ? workspace_bytes : 0);
     LpArgs a{};
@@ -274,11 +452,20 @@ extern "C" int exl3r_token_logprobs(const void* logits, int dtype, int64_t rows,
     a.slices = (int)p.slices;
     a.top = top_k;
     hipStream_t s = (hipStream_t)stream;
-    if (rows * p.slices > 0xffffff) return set_error(EXL3R_EINVAL, "%s: more than 2^24 workgroups", op);
+    const bool vec = aligned16(logits) && a.ld % 16 == 0;
+    if (!p.by_rows && rows * p.slices > 0xffffff) return set_error(EXL3R_EINVAL, "%s: more than 2^24 workgroups", op);
     with_float_type(dtype, [&](auto T) {
         using Ty = decltype(T);
-        launch(k_lp_slices<Ty>, (unsigned)(rows * p.slices), 256, 0, s, a, p.slice);
-        launch(k_lp_rows<Ty>, (unsigned)rows, 256, 0, s, a);
+        if (p.by_rows)
+        {
+            const size_t lds = top_k ? (size_t)p.groups * 4 : 0;
+            if (vec) launch(k_lp_rows<Ty, true>, (unsigned)rows, kLpLanes, lds, s, a);
+            else launch(k_lp_rows<Ty, false>, (unsigned)rows, kLpLanes, lds, s, a);
+            return;
+        }
+        if (vec) launch(k_lp_slices<Ty, true>, (unsigned)(rows * p.slices), kLpLanes, 0, s, a, (int)p.steps);
+        else launch(k_lp_slices<Ty, false>, (unsigned)(rows * p.slices), kLpLanes, 0, s, a, (int)p.steps);
+        launch(k_lp_join<Ty>, (unsigned)rows, kLpLanes, 0, s, a);
     });
     return launch_status(op);
 }

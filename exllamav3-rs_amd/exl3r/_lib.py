@@ -141,7 +141,8 @@ fast = None
 _fast_names = ("exl3r_rms_norm", "exl3r_rms_norm_res_in", "exl3r_silu_mul", "exl3r_gelu_mul", "exl3r_mul_sigmoid",
                "exl3r_gated_rms_norm", "exl3r_gated_rms_norm_had", "exl3r_rope", "exl3r_rope_table", "exl3r_rope_qg",
                "exl3r_rope_paged_kv", "exl3r_rope_paged_kv_had", "exl3r_argmax_sample", "exl3r_gumbel_sample",
-               "exl3r_rms_norm_had", "exl3r_act_mul_had", "exl3r_embedding", "exl3r_embedding_rms_norm")
+               "exl3r_rms_norm_had", "exl3r_act_mul_had", "exl3r_embedding", "exl3r_embedding_rms_norm",
+               "exl3r_paged_attn", "exl3r_paged_attn_shared", "exl3r_token_logprobs")
 
 
 def _bind_fast(lib):

@@ -636,6 +636,12 @@ def paged_attn_workspace_bytes(q, k_cache, block_table, shared_len=0):
 
 def _paged_attn(shared_len, q, k_cache, v_cache, block_table, cache_seqlens, out, scale, window, sinks, lse, workspace,
                 err_flag, stream):
+    if _lib.fast is not None:
+        rc = _lib.fast.paged_attn(shared_len, q, k_cache, v_cache, block_table, cache_seqlens, out, scale, window, sinks, lse,
+                                  workspace, err_flag, stream)
+        if rc is not None:
+            check(rc)
+            return
     if q.dim() != 4 or out.shape != q.shape:
         raise ValueError("q and out must be (bsz, seq_len, heads, head_dim)")
     bsz, seq, hq, hd = q.shape
@@ -703,6 +709,12 @@ def token_logprobs(logits, tokens, logprobs, entropy=None, top_ids=None, top_log
     distribution's entropy, and its top_ids.shape[-1] most probable tokens, ties to the lowest id, with their log
     probabilities, in one read of the logits.  float32 outputs, int64 ids.  workspace: a uint8 tensor of
     token_logprobs_workspace_bytes() bytes (any contents; not shared by calls that overlap)."""
+    if _lib.fast is not None:
+        rc = _lib.fast.token_logprobs(logits, tokens, logprobs, entropy, top_ids, top_logprobs, max_logit, workspace, err_flag,
+                                      stream)
+        if rc is not None:
+            check(rc)
+            return
     rows, vocab, ld = _rows(logits)
     k = 0
     if (tokens is None) != (logprobs is None):

@@ -9,7 +9,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cmath>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/exl3r/rowops.h"
 
@@ -36,6 +38,9 @@ struct Table
     EXL3R_FN(exl3r_act_mul_had);
     EXL3R_FN(exl3r_embedding);
     EXL3R_FN(exl3r_embedding_rms_norm);
+    EXL3R_FN(exl3r_paged_attn);
+    EXL3R_FN(exl3r_paged_attn_shared);
+    EXL3R_FN(exl3r_token_logprobs);
 #undef EXL3R_FN
 } T;
 
@@ -503,6 +508,92 @@ EXL3R_PY(embedding_rms_norm, 10)
                                                         ptr(w), wt, ptr(y), yt, ry.ld, eps, cb, cs, (int32_t*)ptr(err), s); });
 }
 
+// Every tensor on the device of `t`, and that device the current one.
+void same_device(const at::Tensor& t, std::initializer_list<const at::Tensor*> others)
+{
+    need(t.device().index() == c10::hip::current_device());
+    for (const at::Tensor* o : others) need(!o || o->device() == t.device());
+}
+// An optional output of `n` elements, and an optional workspace.
+const at::Tensor* output(PyObject* o, at::ScalarType type, int64_t n)
+{
+    const at::Tensor* t = optional(o);
+    need(!t || (t->scalar_type() == type && t->numel() == n && t->is_contiguous()));
+    return t;
+}
+struct Space
+{
+    const at::Tensor* t;
+    size_t bytes;
+};
+Space space(PyObject* o)
+{
+    const at::Tensor* t = optional(o);
+    need(!t || t->is_contiguous());
+    return { t, t ? t->nbytes() : 0 };
+}
+
+// shared_len (None: exl3r_paged_attn), q, k_cache, v_cache, block_table, cache_seqlens, out, scale, window, sinks, lse,
+// workspace, err_flag, stream
+EXL3R_PY(paged_attn, 14)
+{
+    const auto &q = tensor(v[1]), &out = tensor(v[6]);
+    const Heads Q = heads(q), O = heads(out);
+    need(q.sizes() == out.sizes() && q.numel() > 0);
+    const auto& kc = tensor(v[2]);
+    need(kc.dim() == 4);
+    const Paged p = paged(v + 2, kc.size(2), Q.hd);
+    const int qt = code(q);
+    need(code(kc) == qt && code(p.vc) == qt && code(out) == qt && p.table.size(0) == Q.bsz && p.table.is_contiguous() &&
+         p.lens.numel() == Q.bsz && p.lens.is_contiguous());
+    const auto *lse = output(v[10], at::kFloat, Q.bsz * Q.seq * Q.h), *err = optional(v[12]);
+    const Space ws = space(v[11]);
+    need(!err || err->scalar_type() == at::kInt);
+    same_device(q, { &kc, &p.vc, &p.table, &p.lens, &out, lse, err, ws.t });
+    const float scale = v[7] == Py_None ? (float)(1.0 / std::sqrt((double)Q.hd)) : real(v[7]);
+    const int window = int32_of(v[8]), sinks = int32_of(v[9]);
+    // a batch of one-token sequences may lie at any batch stride
+    const int64_t qs = Q.seq == 1 ? q.stride(0) : Q.ts, os = Q.seq == 1 ? out.stride(0) : O.ts;
+    void* s = stream_of(q, v[13]);
+    if (v[0] == Py_None)
+        return call([&] { return T.exl3r_paged_attn(ptr(q), qs, Q.hs, (int)Q.h, ptr(kc), ptr(p.vc), (int)kc.size(2), (int)kc.size(1),
+                                                    kc.size(0), (const int32_t*)ptr(p.table), p.table.size(1), (const int32_t*)ptr(p.lens),
+                                                    qt, Q.bsz, Q.seq, (int)Q.hd, scale, window, sinks, ptr(out), os, O.hs,
+                                                    (float*)ptr(lse), (int32_t*)ptr(err), ptr(ws.t), ws.bytes, s); });
+    const int64_t shared = whole(v[0]);
+    return call([&] { return T.exl3r_paged_attn_shared(ptr(q), qs, Q.hs, (int)Q.h, ptr(kc), ptr(p.vc), (int)kc.size(2),
+                                                       (int)kc.size(1), kc.size(0), (const int32_t*)ptr(p.table), p.table.size(1),
+                                                       (const int32_t*)ptr(p.lens), shared, qt, Q.bsz, Q.seq, (int)Q.hd, scale,
+                                                       window, sinks, ptr(out), os, O.hs, (float*)ptr(lse), (int32_t*)ptr(err),
+                                                       ptr(ws.t), ws.bytes, s); });
+}
+
+// logits, tokens, logprobs, entropy, top_ids, top_logprobs, max_logit, workspace, err_flag, stream
+EXL3R_PY(token_logprobs, 10)
+{
+    const auto& x = tensor(v[0]);
+    const Rows r = rows_of(x);
+    const auto *tok = output(v[1], at::kLong, r.rows), *lp = output(v[2], at::kFloat, r.rows), *ent = output(v[3], at::kFloat, r.rows);
+    const auto *ids = optional(v[4]), *tl = optional(v[5]), *err = optional(v[8]);
+    need(!tok == !lp && !ids == !tl && (!err || err->scalar_type() == at::kInt));
+    int64_t k = 0;
+    if (ids)
+    {
+        need(ids->dim() > 0 && ids->sizes() == tl->sizes());
+        k = ids->size(-1);
+        need(k > 0 && k <= INT32_MAX);
+        output(v[4], at::kLong, r.rows * k);
+        output(v[5], at::kFloat, r.rows * k);
+    }
+    const Space ws = space(v[7]);
+    same_device(x, { tok, lp, ent, ids, tl, err, ws.t });
+    const int xt = code(x), max_logit = int32_of(v[6]);
+    void* s = stream_of(x, v[9]);
+    return call([&] { return T.exl3r_token_logprobs(ptr(x), xt, r.rows, r.dim, r.ld, max_logit, (const int64_t*)ptr(tok), (float*)ptr(lp),
+                                                    (float*)ptr(ent), (int)k, (int64_t*)ptr(ids), (float*)ptr(tl), (int32_t*)ptr(err),
+                                                    ptr(ws.t), ws.bytes, s); });
+}
+
 // bind(name, address): an entry point of the loaded library.
 PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t k)
 {
@@ -514,7 +605,8 @@ PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t k)
     EXL3R_FN(exl3r_mul_sigmoid) EXL3R_FN(exl3r_gated_rms_norm) EXL3R_FN(exl3r_gated_rms_norm_had) EXL3R_FN(exl3r_rope)
     EXL3R_FN(exl3r_rope_table) EXL3R_FN(exl3r_rope_qg) EXL3R_FN(exl3r_rope_paged_kv) EXL3R_FN(exl3r_rope_paged_kv_had)
     EXL3R_FN(exl3r_argmax_sample) EXL3R_FN(exl3r_gumbel_sample) EXL3R_FN(exl3r_rms_norm_had) EXL3R_FN(exl3r_act_mul_had)
-    EXL3R_FN(exl3r_embedding) EXL3R_FN(exl3r_embedding_rms_norm)
+    EXL3R_FN(exl3r_embedding) EXL3R_FN(exl3r_embedding_rms_norm) EXL3R_FN(exl3r_paged_attn) EXL3R_FN(exl3r_paged_attn_shared)
+    EXL3R_FN(exl3r_token_logprobs)
 #undef EXL3R_FN
     Py_RETURN_FALSE;
 }
@@ -524,6 +616,7 @@ PyMethodDef methods[] = {
     EXL3R_DEF(bind), EXL3R_DEF(rms_norm), EXL3R_DEF(rms_norm_res_in), EXL3R_DEF(act_mul), EXL3R_DEF(gated_rms_norm),
     EXL3R_DEF(gated_rms_norm_had), EXL3R_DEF(rope), EXL3R_DEF(rope_qg), EXL3R_DEF(rope_paged_kv), EXL3R_DEF(rope_paged_kv_had),
     EXL3R_DEF(sample), EXL3R_DEF(rms_norm_had), EXL3R_DEF(act_mul_had), EXL3R_DEF(embedding), EXL3R_DEF(embedding_rms_norm),
+    EXL3R_DEF(paged_attn), EXL3R_DEF(token_logprobs),
     { nullptr, nullptr, 0, nullptr } };
 PyModuleDef module = { PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr };
 
