@@ -52,6 +52,8 @@ struct AttnArgs
     float c;
 };
 
+constexpr float kLn2 = 0.69314718055994530942f;
+
 template <class IO>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
 {
@@ -70,6 +72,12 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c)
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+template <class IO>
+__device__ __forceinline__ float load_bits(uint16_t h)
+{
+    if constexpr (IO::code == DT_F16) return (float)__builtin_bit_cast(_Float16, h);
+    else return bf16lo(h);
+}
 template <class IO>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi)
 {
@@ -101,15 +109,12 @@ __device__ __forceinline__ void wave_lds_fence()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// LDS layout of a tile of K or V: rows of HD elements, the 16-byte chunks of row `key` permuted by an XOR with
-// swz(key), which puts the 16 rows that a K read touches (one chunk column) and the 4 x 64 bytes of a
-// transposing V read on different banks.
-template <int HD>
-__device__ __forceinline__ int swz(int key)
-{
-    if constexpr (HD == 64) return (((key >> 1) & 1) << 2) | ((key >> 2) & 3);
-    else return ((key & 3) << 2) | ((key >> 2) & 3);
-}
+// LDS rows of a tile of K or V are HD elements and a pad that spreads what one read touches over the banks (256 bytes):
+// a K read takes the same 16 bytes of 16 rows, so 16 bytes of pad; a transposing V read takes 64 bytes of 4 rows (MFMA
+// tiles of 32) or 32 bytes of 8 (tiles of 16), so pads of 64 or 32.  Every address is then one register and an offset
+// in the instruction, which an XOR of the chunk index, as free of conflicts, is not.
+template <int HD> constexpr int kRowK = HD * 2 + 16;
+template <int HD, int COLS> constexpr int kRowV = HD * 2 + 2 * COLS;
 
 // A query row: its token and head, its position.
 struct QRow
@@ -180,23 +185,6 @@ __device__ __forceinline__ bool key_seen(const AttnArgs& a, const TileList& l, i
     return j < l.khi && (a.window <= 0 || pmin - j < a.window || j < a.sinks);
 }
 
-// State of 32 query rows (a lane's row, its half of the scores and of o's rows).
-template <int HD>
-struct Acc
-{
-    f32x16 o[HD / 32];
-    float m, l;
-    __device__ __forceinline__ void clear()
-    {
-        #pragma unroll
-        for (int t = 0; t < HD / 32; ++t)
-            #pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-        m = -INFINITY;
-        l = 0.0f;
-    }
-};
-
 // A row's B operand for steps of DK dimensions: part `part` of each step's 8-element parts.
 template <class IO, int HD, int DK>
 __device__ __forceinline__ void load_q(const AttnArgs& a, const QRow& r, int part, u32x4 (&qf)[HD / DK])
@@ -230,20 +218,14 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int64_t tok, int h
     }
 }
 
-// S^T of 32 keys (LDS rows from kb on) and the lane's 32-row column tile.
+// S^T of 32 keys (LDS rows from kb on) and the wave's 32 rows.
 template <class IO, int HD>
 __device__ __forceinline__ f32x16 qk_tile(const char* kb, int lane, const u32x4 (&qf)[HD / 16])
 {
-    const int key = lane & 31, half = lane >> 5;
-    const char* row = kb + key * (HD * 2);
-    const int x = (swz<HD>(key) ^ half) << 4;
+    const char* row = kb + (lane & 31) * kRowK<HD> + (lane >> 5) * 16;
     f32x16 s{};
     #pragma unroll
-    for (int t = 0; t < HD / 16; ++t)
-    {
-        const u32x4 kf = *(const u32x4*)(row + (x ^ (t << 5)));
-        s = mfma32<IO>(kf, qf[t], s);
-    }
+    for (int t = 0; t < HD / 16; ++t) s = mfma32<IO>(*(const u32x4*)(row + t * 32), qf[t], s);
     return s;
 }
 
@@ -262,36 +244,58 @@ __device__ __forceinline__ void mask_tile(f32x16& s, int j0, int half, int p, in
     }
 }
 
-// Exponents of the probabilities are raised by kShift: as f16, whose smallest normal number is 2^-14, a probability
-// keeps its 11 bits down to 2^-28 of the row's largest (bf16 has fp32's range).  o and l carry the same factor.
-template <class IO> constexpr float kShift = IO::code == DT_F16 ? 14.0f : 0.0f;
+// The reference m of a row's exponents is its running maximum, but one that a tile exceeds by less than 2^kSlack stays:
+// o and l are then not rescaled (64 of 185 VALU instructions per tile of 32 keys and 32 rows of 128, where most
+// tiles raise some row's maximum a little).  Exponents are raised by kShift: as f16, whose largest number is below 2^16
+// and smallest normal one 2^-14, a probability then keeps its 11 bits from 2^kSlack of the reference down to 2^-20 of
+// it (bf16 has fp32's range).  o and l carry the same factor.
+constexpr float kSlack = 8.0f;
+template <class IO> constexpr float kShift = IO::code == DT_F16 ? 6.0f : 0.0f;
 
-// The running softmax over one more tile of scores: s becomes the probabilities against the new maximum.
-template <class IO, int HD>
-__device__ __forceinline__ void softmax_tile(Acc<HD>& a, f32x16& s, float c)
+// The factor of o and l when the reference goes from m to mn, and the exponents' constant.
+__device__ __forceinline__ float rescale_factor(float m, float mn, float c)
 {
-    float mx = s[0];
-    #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    const float mn = fmaxf(a.m, max_xor32(mx));
-    const float ref = (mn == -INFINITY ? 0.0f : mn) * c;
-    const float alpha = __builtin_amdgcn_exp2f(fmaf(a.m, c, -ref));
-    float sum = 0.0f;
-    #pragma unroll
-    for (int i = 0; i < 16; ++i)
-    {
-        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, kShift<IO> - ref));
-        sum += s[i];
-    }
-    a.l = fmaf(a.l, alpha, sum);
-    a.m = mn;
-    #pragma unroll
-    for (int t = 0; t < HD / 32; ++t)
-        #pragma unroll
-        for (int i = 0; i < 16; ++i) a.o[t][i] *= alpha;
+    return __builtin_amdgcn_exp2f((m - (mn == -INFINITY ? 0.0f : mn)) * c);
+}
+template <class IO> __device__ __forceinline__ float exponent_base(float m, float c)
+{
+    return kShift<IO> - (m == -INFINITY ? 0.0f : m) * c;
 }
 
-// Whether some of 8 elements of V is an infinity or a NaN.
+// o^T += V^T P^T over 32 keys (LDS rows from vb on).  The probabilities are rounded to V's type for the matrix cores:
+// one rounding of at most half a step each, against the same reference for the whole row; l sums them unrounded.
+template <class IO, int HD>
+__device__ __forceinline__ void pv_tile(f32x16 (&o)[HD / 32], const f32x16& p, const char* vb, int lane)
+{
+    constexpr int RV = kRowV<HD, 32>;
+    const char* r0 = vb + (4 * (lane >> 5) + ((lane >> 2) & 3)) * RV + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    #pragma unroll
+    for (int u = 0; u < 2; ++u)
+    {
+        u32x4 pf;
+        #pragma unroll
+        for (int e = 0; e < 4; ++e) pf[e] = pack2<IO>(p[8 * u + 2 * e], p[8 * u + 2 * e + 1]);
+        #pragma unroll
+        for (int t = 0; t < HD / 32; ++t)
+        {
+            const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + u * 16 * RV + t * 64));
+            const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + (u * 16 + 8) * RV + t * 64));
+            const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+            o[t] = mfma32<IO>(u32x4{ w0.x, w0.y, w1.x, w1.y }, pf, o[t]);
+        }
+    }
+}
+
+// Infinities and NaNs of V in a tile that some row does not see whole: there the probability is 0, but 0 * inf and
+// 0 * NaN must not reach the row.  They are zeroed on their way into LDS, and a workgroup that met one (rare: a bad
+// activation in the cache) adds them at its end, key by key, to the rows that see them.
+template <class IO>
+__device__ __forceinline__ bool nonfinite(uint32_t h)     // 16 bits
+{
+    constexpr uint32_t E = IO::code == DT_F16 ? 0x7c00u : 0x7f80u;
+    return (h & E) == E;
+}
+// Whether some of 8 elements is one.
 template <class IO>
 __device__ __forceinline__ bool nonfinite8(const u32x4& v)
 {
@@ -301,80 +305,12 @@ __device__ __forceinline__ bool nonfinite8(const u32x4& v)
     for (int i = 0; i < 4; ++i) c |= ((v[i] & E2) + B2) & 0x80008000u;
     return c != 0;
 }
-
-// Zeroes the infinities and NaNs of v and returns their indicators: 1 for +inf, 64 for -inf, 65 for a NaN.
 template <class IO>
-__device__ __forceinline__ u32x4 take_nonfinite(u32x4& v)
+__device__ __forceinline__ void zero_nonfinite(u32x4& v)
 {
-    constexpr uint32_t E = IO::code == DT_F16 ? 0x7c00u : 0x7f80u;
-    u32x4 ind;
     #pragma unroll
-    for (int e = 0; e < 4; ++e)
-    {
-        float w[2];
-        uint32_t keep = 0;
-        #pragma unroll
-        for (int k = 0; k < 2; ++k)
-        {
-            const uint32_t h = ((uint32_t)v[e] >> (16 * k)) & 0xffffu, mag = h & 0x7fffu;
-            w[k] = mag > E ? 65.0f : mag < E ? 0.0f : h >> 15 ? 64.0f : 1.0f;
-            keep |= mag < E ? 0xffffu << (16 * k) : 0u;
-        }
-        ind[e] = pack2<IO>(w[0], w[1]);
-        v[e] &= keep;
-    }
-    return ind;
-}
-// What n = (count of +inf) + 64 (count of -inf), NaNs in both, adds to a sum.
-__device__ __forceinline__ float nonfinite_sum(float n)
-{
-    const int c = (int)n;
-    return (c & 63 ? INFINITY : 0.0f) - (c >> 6 ? INFINITY : 0.0f);
-}
-
-// o^T += V^T P^T over 32 keys (LDS rows from vb on).  The probabilities are rounded to V's type for the matrix
-// cores: one rounding of at most half a step each, against the same maximum for the whole row; l sums them
-// unrounded.  CARE: V has infinities or NaNs and some row does not see some of these keys; there the probability
-// is 0, but 0 * inf and 0 * NaN must not reach the row.  They are then taken out of the product and applied by a
-// second one, of 1 where V has +inf or NaN, 64 where it has -inf or NaN and 65 for a NaN, with "the row's probability
-// is not 0": its sums over at most 32 keys tell how many of each a row sees.
-template <class IO, int HD, bool CARE>
-__device__ __forceinline__ void pv_tile(Acc<HD>& a, const f32x16& p, const char* vb, int lane)
-{
-    const int i16 = lane & 15, half = lane >> 5;
-    const int key = 4 * half + (i16 >> 2);
-    const int c0 = ((lane >> 3) & 2) | ((i16 >> 1) & 1);
-    const char* r0 = vb + key * (HD * 2) + ((i16 & 1) << 3);
-    const int x0 = (swz<HD>(key) ^ c0) << 4, x1 = (swz<HD>(key + 8) ^ c0) << 4;
-    #pragma unroll
-    for (int u = 0; u < 2; ++u)
-    {
-        u32x4 pf, see{};
-        #pragma unroll
-        for (int e = 0; e < 4; ++e)
-        {
-            pf[e] = pack2<IO>(p[8 * u + 2 * e], p[8 * u + 2 * e + 1]);
-            if constexpr (CARE)
-                see[e] = pack2<IO>(p[8 * u + 2 * e] != 0.0f ? 1.0f : 0.0f, p[8 * u + 2 * e + 1] != 0.0f ? 1.0f : 0.0f);
-        }
-        #pragma unroll
-        for (int t = 0; t < HD / 32; ++t)
-        {
-            const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + u * 16 * HD * 2 + (x0 ^ (t << 6))));
-            const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + (u * 16 + 8) * HD * 2 + (x1 ^ (t << 6))));
-            const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-            u32x4 vf = { w0.x, w0.y, w1.x, w1.y };
-            if constexpr (CARE)
-            {
-                const u32x4 ind = take_nonfinite<IO>(vf);
-                f32x16 n{};
-                n = mfma32<IO>(ind, see, n);
-                #pragma unroll
-                for (int i = 0; i < 16; ++i) a.o[t][i] += nonfinite_sum(n[i]);
-            }
-            a.o[t] = mfma32<IO>(vf, pf, a.o[t]);
-        }
-    }
+    for (int i = 0; i < 4; ++i)
+        v[i] &= (nonfinite<IO>(v[i]) ? 0u : 0xffffu) | (nonfinite<IO>(v[i] >> 16) ? 0u : 0xffff0000u);
 }
 
 // The page of key j (-1 past the keys of the launch).
@@ -422,6 +358,60 @@ __device__ __forceinline__ void load_tile(const AttnArgs& a, int j0, int entry, 
     }
 }
 
+// A tile into LDS: keys that the launch must not see as zeros and, where not every row sees all of it (`part`),
+// without V's infinities and NaNs.  Returns whether there were such.
+template <class IO, int HD, int STEPS, int LANES, int RV>
+__device__ __forceinline__ bool write_tile(u32x4 (&ks)[STEPS], u32x4 (&vs)[STEPS], uint64_t ok, bool part, int lane_of_tile,
+                                           char* kl, char* vl)
+{
+    constexpr int CH = HD / 8, KPS = LANES / CH;
+    const int key = lane_of_tile / CH, ch = lane_of_tile % CH;
+    bool odd = false;
+    if (part)
+    {
+        #pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+        {
+            if (!((ok >> (k * KPS + key)) & 1)) ks[k] = vs[k] = u32x4{};
+            if (nonfinite8<IO>(vs[k]))
+            {
+                zero_nonfinite<IO>(vs[k]);
+                odd = true;
+            }
+        }
+    }
+    char* const kd = kl + key * kRowK<HD> + ch * 16;
+    char* const vd = vl + key * RV + ch * 16;
+    #pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+    {
+        *(u32x4*)(kd + k * KPS * kRowK<HD>) = ks[k];
+        *(u32x4*)(vd + k * KPS * RV) = vs[k];
+    }
+    return odd;
+}
+
+// Calls add(j, v) for every key j of the tile at j0 with V's row there (global memory).
+template <int HD, class F>
+__device__ __forceinline__ void each_value_row(const AttnArgs& a, const TileList& l, const int32_t* table, int j0, int keys, int kvh, F&& add)
+{
+    for (int j = j0; j < j0 + keys && j < l.khi; ++j)
+    {
+        const int page = table[j >> a.page_shift];
+        if ((uint64_t)(int64_t)page >= (uint64_t)a.num_pages) continue;
+        const int64_t row = ((int64_t)page << a.page_shift) + (j & ((1 << a.page_shift) - 1));
+        add(j, (gcptr<uint16_t>)a.vc + (row * a.hk + kvh) * HD);
+    }
+}
+__device__ __forceinline__ bool row_sees(const AttnArgs& a, int p, int j)
+{
+    return j <= p && (a.window <= 0 || p - j < a.window || j < a.sinks);
+}
+// Whether every row with a position in [pmin, pmax] sees all of the keys j .. j + n - 1.
+__device__ __forceinline__ bool all_seen(const AttnArgs& a, int j, int n, int pmin, int pmax)
+{
+    return j + n - 1 <= pmin && (a.window <= 0 || pmax - j < a.window || j + n - 1 < a.sinks);
+}
 // The launch's item: KV head (fastest: consecutive workgroups go to different XCDs, so with 8 KV heads an XCD's
 // L2 holds the keys of one head), then row tile (the last, longest first), split, row set.
 struct Item
@@ -448,141 +438,171 @@ __device__ __forceinline__ void flag_positions(const AttnArgs& a, const QRow& r)
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many query rows: 4 waves of NQ * 32 rows each share tiles of 64 keys in LDS; the next tile's loads are in
-// flight (registers) while a tile is multiplied.
-template <class IO, int HD, int NQ, bool SMALL>
-__global__ __launch_bounds__(256, HD == 256 || NQ == 2 ? 1 : 2) void k_attn_rows(AttnArgs a)
+// Many query rows: WAVES waves of 32 rows each share tiles of KT keys in a ring of three LDS stages.  While a tile's
+// scores become probabilities (VALU), the matrix cores are at the next tile's scores; the tile after that is on its
+// way into the third stage, and the one after it in registers.  One barrier per tile.
+template <class IO, int HD, int WAVES, int KT, bool SMALL>
+__global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
 {
-    constexpr int KT = 64, CH = HD / 8, RB = HD * 2, STEPS = KT * CH / 256;
-    __shared__ __align__(16) char lds[2 * KT * RB];
-    char* const kl = lds;
-    char* const vl = lds + KT * RB;
+    constexpr int LANES = WAVES * 64, RK = kRowK<HD>, RV = kRowV<HD, 32>, STEPS = KT * (HD / 8) / LANES, NS = KT / 32;
+    constexpr int STAGE = KT * (RK + RV);
+    __shared__ __align__(16) char lds[3 * STAGE];
+    __shared__ int plo[WAVES], phi[WAVES], odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const Item it = launch_item(a);
-
-    QRow row[NQ];
-    u32x4 qf[NQ][HD / 16];
-    Acc<HD> acc[NQ];
-    int pmin[NQ], pmax[NQ];
-    const int r0 = it.tile * (128 * NQ) + wave * (32 * NQ);
-    #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-    {
-        row[n] = query_row(a, it.set, it.kvh, min(r0 + 32 * n + (lane & 31), a.rows - 1));
-        load_q<IO, HD, 16>(a, row[n], half, qf[n]);
-        acc[n].clear();
-        pmin[n] = wave_min(row[n].p);
-        pmax[n] = wave_max(row[n].p);
-        if (it.split == 0 && it.kvh == 0) flag_positions(a, row[n]);
-    }
-    // positions of the whole workgroup's rows
-    __shared__ int plo[4], phi[4], odd[2];
-    int wmin = pmin[0], wmax = pmax[0];
-    #pragma unroll
-    for (int n = 1; n < NQ; ++n) { wmin = min(wmin, pmin[n]); wmax = max(wmax, pmax[n]); }
-    if (lane == 0) { plo[wave] = wmin; phi[wave] = wmax; }
-    if (tid == 0) odd[0] = odd[1] = 0;
+    const int r0 = it.tile * (32 * WAVES) + wave * 32;
+    const QRow row = query_row(a, it.set, it.kvh, min(r0 + (lane & 31), a.rows - 1));
+    if (it.split == 0 && it.kvh == 0) flag_positions(a, row);
+    const int pmin = wave_min(row.p), pmax = wave_max(row.p);
+    if (lane == 0) { plo[wave] = pmin; phi[wave] = pmax; }
+    if (tid == 0) odd = 0;
+    u32x4 qf[HD / 16];
+    load_q<IO, HD, 16>(a, row, half, qf);
     __syncthreads();
-    const int gmin = min(min(plo[0], plo[1]), min(plo[2], plo[3]));
-    const int gmax = max(max(phi[0], phi[1]), max(phi[2], phi[3]));
+    int gmin = plo[0], gmax = phi[0];       // positions of the workgroup's rows
+    #pragma unroll
+    for (int w = 1; w < WAVES; ++w) { gmin = min(gmin, plo[w]); gmax = max(gmax, phi[w]); }
+    gmin = __builtin_amdgcn_readfirstlane(gmin);
+    gmax = __builtin_amdgcn_readfirstlane(gmax);
     const TileList tl = tile_list(a, gmin, gmax, KT);
     const int per = (tl.count + a.nsplit - 1) / a.nsplit;
     const int t0 = min(it.split * per, tl.count), t1 = min(t0 + per, tl.count);
-
     const int32_t* table = a.table + (a.whole ? 0 : (int64_t)it.set * a.max_blocks);
+    const auto tile_key = [&](int i) { return a.dom_lo + tl.tile(i) * KT; };
+
+    f32x16 o[HD / 32];
+    #pragma unroll
+    for (int t = 0; t < HD / 32; ++t) o[t] = f32x16{};
+    float m = -INFINITY, l = 0.0f;
+
     u32x4 ks[STEPS], vs[STEPS];
     int entry = -1;
-    uint64_t ok_next = 0;
-    auto fetch_entry = [&](int i) { entry = i < t1 ? page_entry(a, table, a.dom_lo + tl.tile(i) * KT + lane, tl.khi) : -1; };
-    auto stage = [&](int i) {
-        const int j0 = a.dom_lo + tl.tile(i) * KT;
-        const bool in = key_seen(a, tl, j0 + lane, gmin), good = in && (uint64_t)(int64_t)entry < (uint64_t)a.num_pages;
+    uint64_t ok_load = 0;      // of the tile in registers
+    const auto fetch_entry = [&](int i) { entry = i < t1 ? page_entry(a, table, tile_key(i) + (lane & (KT - 1)), tl.khi) : -1; };
+    const auto load = [&](int i) {
+        if (i >= t1) return;
+        const int j0 = tile_key(i);
+        const bool in = key_seen(a, tl, j0 + (lane & (KT - 1)), gmin), good = in && (uint64_t)(int64_t)entry < (uint64_t)a.num_pages;
         if (a.err && in && !good) *a.err = 1;
-        ok_next = __ballot(good);
-        load_tile<HD, SMALL, STEPS, 256>(a, j0, entry, ok_next, it.kvh, tid, ks, vs);
+        ok_load = __ballot(good);
+        if (KT == 32) ok_load &= 0xffffffffu;
+        load_tile<HD, SMALL, STEPS, LANES>(a, j0, entry, ok_load, it.kvh, tid, ks, vs);
+        fetch_entry(i + 1);
     };
+    constexpr uint64_t FULL = KT == 64 ? ~0ull : 0xffffffffull;
+    const auto write = [&](int i) {      // the tile in registers into its stage
+        if (i >= t1) return;
+        char* const st = lds + ((i - t0) % 3) * STAGE;
+        const bool part = ok_load != FULL || !all_seen(a, tile_key(i), KT, gmin, gmax);
+        if (write_tile<IO, HD, STEPS, LANES, RV>(ks, vs, ok_load, part, tid, st, st + KT * RK)) odd = 1;
+    };
+    uint64_t ok_now = 0, ok_next = 0;    // of tiles i and i + 1
     fetch_entry(t0);
-    if (t0 < t1) { stage(t0); fetch_entry(t0 + 1); }
-    for (int i = t0; i < t1; ++i)
+    load(t0);
+    write(t0);
+    ok_now = ok_load;
+    load(t0 + 1);
+    __syncthreads();
+    f32x16 sa[NS], sb[NS];
+    const auto scores = [&](int i, f32x16 (&s)[NS]) {
+        const char* const st = lds + ((i - t0) % 3) * STAGE;
+        #pragma unroll
+        for (int k = 0; k < NS; ++k) s[k] = qk_tile<IO, HD>(st + k * 32 * RK, lane, qf);
+    };
+    if (t0 < t1) scores(t0, sa);
+    write(t0 + 1);
+    ok_next = ok_load;
+    load(t0 + 2);
+    __syncthreads();
+    const float slack = kSlack / a.c;
+    // Tile i, whose scores are in s; the next tile's go to sn.
+    const auto step = [&](int i, f32x16 (&s)[NS], f32x16 (&sn)[NS]) __attribute__((always_inline)) {
+        const int j0 = tile_key(i);
+        const char* const st = lds + ((i - t0) % 3) * STAGE;
+        if (ok_now != FULL || !all_seen(a, j0, KT, pmin, pmax))
+        {
+            #pragma unroll
+            for (int k = 0; k < NS; ++k)
+                mask_tile(s[k], j0 + 32 * k, half, row.p, a.window, a.sinks, (uint32_t)(ok_now >> (32 * k)));
+        }
+        float mx = s[0][0];
+        #pragma unroll
+        for (int k = 0; k < NS; ++k)
+            #pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][e]);
+        mx = max_xor32(mx);
+        if (__any(mx > m + slack))
+        {
+            const float mn = fmaxf(m, mx), alpha = rescale_factor(m, mn, a.c);
+            l *= alpha;
+            m = mn;
+            #pragma unroll
+            for (int t = 0; t < HD / 32; ++t)
+                #pragma unroll
+                for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
+        }
+        scores(i + 1, sn);
+        const float base = exponent_base<IO>(m, a.c);
+        float sum[4] = {};
+        #pragma unroll
+        for (int k = 0; k < NS; ++k)
+            #pragma unroll
+            for (int e = 0; e < 16; ++e)
+            {
+                s[k][e] = __builtin_amdgcn_exp2f(fmaf(s[k][e], a.c, base));
+                sum[e & 3] += s[k][e];
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        #pragma unroll
+        for (int k = 0; k < NS; ++k) pv_tile<IO, HD>(o, s[k], st + KT * RK + k * 32 * RV, lane);
+        write(i + 2);
+        ok_now = ok_next;
+        ok_next = ok_load;
+        load(i + 3);
+        __syncthreads();
+    };
+    for (int i = t0; i < t1; i += 2)
     {
-        const uint64_t ok = ok_next;
-        const int j0 = a.dom_lo + tl.tile(i) * KT;
-        const bool all = ok == ~0ull && j0 + KT - 1 <= gmin && (a.window <= 0 || gmax - j0 < a.window || j0 + KT - 1 < a.sinks);
-        __syncthreads();
-        bool nf = false;
-        if (!all)
-        {
-            #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-            {
-                if (!((ok >> ((k * 256 + tid) / CH)) & 1)) ks[k] = vs[k] = u32x4{};
-                nf |= nonfinite8<IO>(vs[k]);
-            }
-        }
-        #pragma unroll
-        for (int k = 0; k < STEPS; ++k)
-        {
-            const int slot = k * 256 + tid, key = slot / CH, ch = slot % CH;
-            const int at = key * RB + ((ch ^ swz<HD>(key)) << 4);
-            *(u32x4*)(kl + at) = ks[k];
-            *(u32x4*)(vl + at) = vs[k];
-        }
-        // odd[i & 1]: V of this tile has infinities or NaNs and not every row sees all of it
-        if (nf) odd[i & 1] = 1;
-        if (tid == 0) odd[(i + 1) & 1] = 0;
-        __syncthreads();
-        const bool care = odd[i & 1] != 0;
-        if (i + 1 < t1) { stage(i + 1); fetch_entry(i + 2); }
-        #pragma unroll
-        for (int n = 0; n < NQ; ++n)
-        {
-            #pragma unroll
-            for (int k = 0; k < 2; ++k)
-            {
-                const int j = j0 + 32 * k;
-                const uint32_t okw = (uint32_t)(ok >> (32 * k));
-                const bool none = okw == 0 || j > pmax[n] || (a.window > 0 && pmin[n] - (j + 31) >= a.window && j >= a.sinks);
-                if (none) continue;
-                const bool whole = okw == 0xffffffffu && j + 31 <= pmin[n] &&
-                                   (a.window <= 0 || pmax[n] - j < a.window || j + 31 < a.sinks);
-                f32x16 s = qk_tile<IO, HD>(kl + k * 32 * RB, lane, qf[n]);
-                if (!whole) mask_tile(s, j, half, row[n].p, a.window, a.sinks, okw);
-                softmax_tile<IO, HD>(acc[n], s, a.c);
-                if (!care) pv_tile<IO, HD, false>(acc[n], s, vl + k * 32 * RB, lane);
-                else pv_tile<IO, HD, true>(acc[n], s, vl + k * 32 * RB, lane);
-            }
-        }
+        step(i, sa, sb);
+        if (i + 1 < t1) step(i + 1, sb, sa);
     }
-    #pragma unroll
-    for (int n = 0; n < NQ; ++n)
+    if (odd)
+        for (int i = t0; i < t1; ++i)
+            each_value_row<HD>(a, tl, table, tile_key(i), KT, it.kvh, [&](int j, gcptr<uint16_t> v) {
+                #pragma unroll
+                for (int t = 0; t < HD / 32; ++t)
+                    #pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                    {
+                        const uint16_t h = v[32 * t + 8 * (e / 4) + 4 * half + e % 4];
+                        if (nonfinite<IO>(h) && row_sees(a, row.p, j)) o[t][e] += load_bits<IO>(h);
+                    }
+            });
+    l = sum_xor32(l);
+    if (r0 + (lane & 31) >= a.rows) return;
+    const int64_t gr = row.tok * a.hq + row.h;
+    if (a.direct)
     {
-        const int r = r0 + 32 * n + (lane & 31);
-        const float l = sum_xor32(acc[n].l);
-        if (r >= a.rows) continue;
-        const int64_t gr = row[n].tok * a.hq + row[n].h;
-        if (a.direct)
-        {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (a.lse && half == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (fmaf(acc[n].m, a.c, -kShift<IO>) + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        if (a.lse && half == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (fmaf(m, a.c, -kShift<IO>) + __builtin_amdgcn_logf(l)) * kLn2;
+        #pragma unroll
+        for (int t = 0; t < HD / 32; ++t)
             #pragma unroll
-            for (int t = 0; t < HD / 32; ++t)
-                #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    store_out4<IO>(a, row[n].tok, row[n].h, 32 * t + 8 * g + 4 * half, acc[n].o[t][4 * g] * inv,
-                                   acc[n].o[t][4 * g + 1] * inv, acc[n].o[t][4 * g + 2] * inv, acc[n].o[t][4 * g + 3] * inv);
-        }
-        else
-        {
-            const int64_t pr = gr * a.splits + a.split0 + it.split;
-            if (half == 0) { a.pml[2 * pr] = fmaf(acc[n].m, a.c, -kShift<IO>); a.pml[2 * pr + 1] = l; }
-            if (l == 0.0f) continue;
-            gptr<f32x4> d = (gptr<f32x4>)(a.po + pr * HD + 4 * half);
+            for (int g = 0; g < 4; ++g)
+                store_out4<IO>(a, row.tok, row.h, 32 * t + 8 * g + 4 * half, o[t][4 * g] * inv, o[t][4 * g + 1] * inv,
+                               o[t][4 * g + 2] * inv, o[t][4 * g + 3] * inv);
+    }
+    else
+    {
+        const int64_t pr = gr * a.splits + a.split0 + it.split;
+        if (half == 0) { a.pml[2 * pr] = fmaf(m, a.c, -kShift<IO>); a.pml[2 * pr + 1] = l; }
+        if (l == 0.0f) return;
+        gptr<f32x4> d = (gptr<f32x4>)(a.po + pr * HD + 4 * half);
+        #pragma unroll
+        for (int t = 0; t < HD / 32; ++t)
             #pragma unroll
-            for (int t = 0; t < HD / 32; ++t)
-                #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    d[8 * t + 2 * g] = f32x4{ acc[n].o[t][4 * g], acc[n].o[t][4 * g + 1], acc[n].o[t][4 * g + 2], acc[n].o[t][4 * g + 3] };
-        }
+            for (int g = 0; g < 4; ++g)
+                d[8 * t + 2 * g] = f32x4{ o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3] };
     }
 }
 
@@ -595,12 +615,12 @@ __global__ __launch_bounds__(256, HD == 256 || NQ == 2 ? 1 : 2) void k_attn_rows
 template <class IO, int HD, int NC, bool SMALL>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a)
 {
-    constexpr int KT = 32, CH = HD / 8, RB = HD * 2, STEPS = KT * CH / 64, ROWS = 16 * NC;
-    __shared__ __align__(16) char lds[4][2 * KT * RB];
+    constexpr int KT = 32, RK = kRowK<HD>, RV = kRowV<HD, 16>, STEPS = KT * (HD / 8) / 64, ROWS = 16 * NC;
+    __shared__ __align__(16) char lds[4][KT * (RK + RV)];
     __shared__ float mlw[4][2][ROWS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, col = lane & 15;
     char* const kl = lds[wave];
-    char* const vl = lds[wave] + KT * RB;
+    char* const vl = lds[wave] + KT * RK;
     const Item it = launch_item(a);
     const int r0 = it.tile * ROWS;
     QRow row[NC];
@@ -649,36 +669,17 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         l[n] = 0.0f;
     }
     // K fragment: key row col (of 16), chunks 4 t + quad; V^T fragment: keys 4 quad + 0..3 (and + 16), columns 16 t + col
-    const char* const krow = kl + col * RB;
-    const int kx = (swz<HD>(col) ^ quad) << 4;
-    const int vkey = 4 * quad + (col >> 2);
-    const char* const vrow = vl + vkey * RB + ((col & 1) << 3);
-    const int vx = (swz<HD>(vkey) ^ ((col >> 1) & 1)) << 4;
+    const char* const krow = kl + col * RK + quad * 16;
+    const char* const vrow = vl + (4 * quad + (col >> 2)) * RV + (col & 3) * 8;
+    const float slack = kSlack / a.c;
+    bool odd = false;
     for (int i = t0 + wave; i < t1; i += 4)
     {
         const uint32_t ok = ok_next;
         const int j = a.dom_lo + tl.tile(i) * KT;
-        const bool whole = ok == 0xffffffffu && j + 31 <= pmin && (a.window <= 0 || pmax - j < a.window || j + 31 < a.sinks);
-        bool nf = false;
+        const bool whole = ok == 0xffffffffu && all_seen(a, j, KT, pmin, pmax);
         wave_lds_fence();
-        if (!whole)
-        {
-            #pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-            {
-                if (!((ok >> ((k * 64 + lane) / CH)) & 1)) ks[k] = vs[k] = u32x4{};
-                nf |= nonfinite8<IO>(vs[k]);
-            }
-        }
-        #pragma unroll
-        for (int k = 0; k < STEPS; ++k)
-        {
-            const int slot = k * 64 + lane, key = slot / CH, ch = slot % CH;
-            const int at = key * RB + ((ch ^ swz<HD>(key)) << 4);
-            *(u32x4*)(kl + at) = ks[k];
-            *(u32x4*)(vl + at) = vs[k];
-        }
-        const bool care = __any(nf);
+        odd |= write_tile<IO, HD, STEPS, 64, RV>(ks, vs, ok, !whole, lane, kl, vl);
         wave_lds_fence();
         if (i + 4 < t1) { stage(i + 4); fetch_entry(i + 8); }
         if (ok == 0) continue;
@@ -691,12 +692,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
             #pragma unroll
             for (int t = 0; t < HD / 32; ++t)
             {
-                const u32x4 kf = *(const u32x4*)(krow + k * 16 * RB + (kx ^ (t << 6)));
+                const u32x4 kf = *(const u32x4*)(krow + k * 16 * RK + t * 64);
                 #pragma unroll
                 for (int n = 0; n < NC; ++n) s[n][k] = mfma16<IO>(kf, qf[n][t], s[n][k]);
             }
         }
-        u32x4 pf[NC], see[NC];
+        u32x4 pf[NC];
         #pragma unroll
         for (int n = 0; n < NC; ++n)
         {
@@ -717,51 +718,55 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
             float mx = s[n][0][0];
             #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[n][e >> 2][e & 3]);
-            const float mn = fmaxf(m[n], max_xor32(max_xor16(mx)));
-            const float ref = (mn == -INFINITY ? 0.0f : mn) * a.c;
-            const float alpha = __builtin_amdgcn_exp2f(fmaf(m[n], a.c, -ref));
+            mx = max_xor32(max_xor16(mx));
+            if (__any(mx > m[n] + slack))
+            {
+                const float mn = fmaxf(m[n], mx), alpha = rescale_factor(m[n], mn, a.c);
+                l[n] *= alpha;
+                m[n] = mn;
+                #pragma unroll
+                for (int t = 0; t < HD / 16; ++t)
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][t][e] *= alpha;
+            }
+            const float base = exponent_base<IO>(m[n], a.c);
             float sum = 0.0f, pr[8];
             #pragma unroll
             for (int e = 0; e < 8; ++e)
             {
-                pr[e] = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], a.c, kShift<IO> - ref));
+                pr[e] = __builtin_amdgcn_exp2f(fmaf(s[n][e >> 2][e & 3], a.c, base));
                 sum += pr[e];
             }
-            l[n] = fmaf(l[n], alpha, sum);
-            m[n] = mn;
+            l[n] += sum;
             #pragma unroll
-            for (int e = 0; e < 4; ++e)
-            {
-                pf[n][e] = pack2<IO>(pr[2 * e], pr[2 * e + 1]);
-                see[n][e] = pack2<IO>(pr[2 * e] != 0.0f ? 1.0f : 0.0f, pr[2 * e + 1] != 0.0f ? 1.0f : 0.0f);
-            }
-            #pragma unroll
-            for (int t = 0; t < HD / 16; ++t)
-                #pragma unroll
-                for (int e = 0; e < 4; ++e) o[n][t][e] *= alpha;
+            for (int e = 0; e < 4; ++e) pf[n][e] = pack2<IO>(pr[2 * e], pr[2 * e + 1]);
         }
         #pragma unroll
         for (int t = 0; t < HD / 16; ++t)
         {
-            const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(vrow + (vx ^ (t << 5))));
-            const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(vrow + 16 * RB + (vx ^ (t << 5))));
+            const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(vrow + t * 32));
+            const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(vrow + 16 * RV + t * 32));
             const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-            u32x4 vf = { w0.x, w0.y, w1.x, w1.y };
-            if (care)
-            {
-                const u32x4 ind = take_nonfinite<IO>(vf);
-                #pragma unroll
-                for (int n = 0; n < NC; ++n)
-                {
-                    const f32x4 c = mfma16<IO>(ind, see[n], f32x4{});
-                    #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[n][t][e] += nonfinite_sum(c[e]);
-                }
-            }
+            const u32x4 vf = { w0.x, w0.y, w1.x, w1.y };
             #pragma unroll
             for (int n = 0; n < NC; ++n) o[n][t] = mfma16<IO>(vf, pf[n], o[n][t]);
         }
     }
+    if (__any(odd))
+        for (int i = t0 + wave; i < t1; i += 4)
+            each_value_row<HD>(a, tl, table, a.dom_lo + tl.tile(i) * KT, KT, it.kvh, [&](int j, gcptr<uint16_t> v) {
+                #pragma unroll
+                for (int t = 0; t < HD / 16; ++t)
+                    #pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        const uint16_t h = v[16 * t + 4 * quad + e];
+                        if (!nonfinite<IO>(h)) continue;
+                        #pragma unroll
+                        for (int n = 0; n < NC; ++n)
+                            if (row_sees(a, row[n].p, j)) o[n][t][e] += load_bits<IO>(h);
+                    }
+            });
     // Join the waves: o against the common maximum, through LDS as [row][HD] floats with the 16-byte chunks of a
     // row permuted by its low bits.
     float lw[NC];
@@ -780,7 +785,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         #pragma unroll
         for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mlw[w][0][r]);
         const float ref = (mm == -INFINITY ? 0.0f : mm) * a.c;
-        const float f = __builtin_amdgcn_exp2f(fmaf(m[n], a.c, -ref));
+        // (kept above 0: an infinity of o stays one)
+        const float f = fmaxf(__builtin_amdgcn_exp2f(fmaf(m[n], a.c, -ref)), 0x1p-126f);
         #pragma unroll
         for (int t = 0; t < HD / 16; ++t)
         {
@@ -815,7 +821,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         if (a.direct)
         {
             const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-            if (a.lse && ch == 0) a.lse[gr] = ls == 0.0f ? -INFINITY : (rf - kShift<IO> + __builtin_amdgcn_logf(ls)) * 0.69314718055994530942f;
+            if (a.lse && ch == 0) a.lse[gr] = ls == 0.0f ? -INFINITY : (rf - kShift<IO> + __builtin_amdgcn_logf(ls)) * kLn2;
             store_out4<IO>(a, qr.tok, qr.h, 4 * ch, sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
         }
         else
@@ -850,7 +856,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a)
     for (int i = lane; i < ns; i += 64)
     {
         const f32x2 e = ml[i];
-        const float w = e.y != 0.0f ? __builtin_amdgcn_exp2f(e.x - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+        const float w = fmaxf(__builtin_amdgcn_exp2f(e.x - (m == -INFINITY ? 0.0f : m)), 0x1p-126f);   // as f above
         if (sub == 0) wt[local][i] = e.y != 0.0f ? w : -1.0f;      // -1: nothing was written
         if (e.y != 0.0f) l = fmaf(w, e.y, l);
     }
@@ -883,7 +889,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a)
     const int64_t tok = gr / a.hq;
     const int h = (int)(gr - tok * a.hq);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (a.lse && lane == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * 0.69314718055994530942f;
+    if (a.lse && lane == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     store_out4<IO>(a, tok, h, 4 * lane, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
@@ -900,13 +906,14 @@ struct Phase
 };
 
 // How a phase is cut: `sets` row sets of `rows` query rows per KV head against at most `span` keys.
-Phase plan_phase(int64_t sets, int64_t rows, int hk, int64_t span)
+Phase plan_phase(int64_t sets, int64_t rows, int hk, int hd, int64_t span)
 {
     Phase p;
-    p.cols = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+    // (two column tiles of 256 dimensions do not fit the registers: two row tiles then, whose keys meet in the L2)
+    p.cols = rows > 32 ? 0 : rows <= 16 || hd == 256 ? 1 : 2;
     p.sets = sets;
     p.rows = rows;
-    const int64_t per_tile = p.cols ? 16 * p.cols : 128;
+    const int64_t per_tile = p.cols ? 16 * p.cols : hd == 256 ? 128 : 256;
     p.row_tiles = (rows + per_tile - 1) / per_tile;
     const int64_t base = sets * hk * p.row_tiles;
     const int64_t want = p.cols ? 4096 : 512, least = p.cols ? 128 : 256;
@@ -936,8 +943,8 @@ Plan make_plan(int64_t bsz, int64_t seq, int hq, int hk, int hd, int64_t cap, in
         const int64_t w = window + seq + sinks + 256;
         if (w < span) span = w;
     }
-    p.own = plan_phase(bsz, seq * group, hk, span);
-    if (shared > 0) p.prefix = plan_phase(1, bsz * seq * group, hk, shared);
+    p.own = plan_phase(bsz, seq * group, hk, hd, span);
+    if (shared > 0) p.prefix = plan_phase(1, bsz * seq * group, hk, hd, shared);
     p.splits = p.own.nsplit + p.prefix.nsplit;
     p.join = p.splits > 1;
     if (p.join) p.bytes = ((size_t)p.splits * (size_t)(bsz * seq * hq) * (size_t)(hd + 2) * 4 + 255) & ~(size_t)255;
@@ -1023,15 +1030,16 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
             const int64_t grid = ph.sets * hk * ph.row_tiles * ph.nsplit;
             if (ph.cols == 0)
             {
-                if (page_size < 64) launch(k_attn_rows<IO, HD, 1, true>, (unsigned)grid, 256, 0, st, x);
-                else launch(k_attn_rows<IO, HD, 1, false>, (unsigned)grid, 256, 0, st, x);
+                constexpr int W = HD == 256 ? 4 : 8, KT = HD == 256 ? 32 : 64;
+                if (page_size < KT) launch(k_attn_rows<IO, HD, W, KT, true>, (unsigned)grid, 64 * W, 0, st, x);
+                else launch(k_attn_rows<IO, HD, W, KT, false>, (unsigned)grid, 64 * W, 0, st, x);
             }
             else if (ph.cols == 1)
             {
                 if (page_size < 32) launch(k_attn_keys<IO, HD, 1, true>, (unsigned)grid, 256, 0, st, x);
                 else launch(k_attn_keys<IO, HD, 1, false>, (unsigned)grid, 256, 0, st, x);
             }
-            else
+            else if constexpr (HD != 256)
             {
                 if (page_size < 32) launch(k_attn_keys<IO, HD, 2, true>, (unsigned)grid, 256, 0, st, x);
                 else launch(k_attn_keys<IO, HD, 2, false>, (unsigned)grid, 256, 0, st, x);

@@ -7,7 +7,8 @@ W = sum_j w_j |v_j|:
     products, off by at most (head_dim + 2) 2^-24 scale sum_d |q_d k_d| =: d (natural units), its exponent in base 2
     and the exponential by 2^-22 + 2^-23 |s - m|: a weight is off by the relative u + e, the sum of the weights by e,
     e = 2 d + 2^-21 + 2^-22 max|s - m|;  with 2^-19 for the fp32 sums: (u + 2 e + 2^-19) W;
-  - f16 weights below 2^-28 of the row's largest have an absolute error of 2^-39 of it instead: 2^-39 sum_j |v_j|
+  - f16 weights are held as 2^6 times their ratio to a reference that is at most the row's largest weight, so below 2^-20
+    of it they have, instead, an absolute error of half of f16's smallest denormal, 2^-25, over 2^6: 2^-31 sum_j |v_j|
     (the softmax's sum is at least the largest weight);
   - out is rounded once: u |out|, and by at most half its smallest denormal.
 lse is off by e, its own rounding 2^-23 |lse| and the fp32 sum."""
@@ -94,7 +95,7 @@ def exact(q, kc, vc, table, lens, window=0, sinks=0, scale=None, bad_pages=()):
             W = (w[:, :, None] * vv.abs()).sum(1)
             tol[b, :, h] = (u + 2 * e + 2.0 ** -19)[:, None] * W
             if q.dtype == F16:
-                tol[b, :, h] += 2.0 ** -39 * vv.abs().sum(1) + 2.0 ** -25
+                tol[b, :, h] += 2.0 ** -31 * vv.abs().sum(1) + 2.0 ** -25
             tol_lse[b, :, h] = e + 2.0 ** -19 + 2.0 ** -23 * z.abs()
     return out, lse, tol + u * out.abs(), tol_lse
 
