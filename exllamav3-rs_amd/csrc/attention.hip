@@ -218,15 +218,11 @@ __device__ __forceinline__ void store_out4(const AttnArgs& a, int64_t tok, int h
     }
 }
 
-// S^T of 32 keys (LDS rows from kb on) and the wave's 32 rows.
-template <class IO, int HD>
-__device__ __forceinline__ f32x16 qk_tile(const char* kb, int lane, const u32x4 (&qf)[HD / 16])
+// K fragment of 32 keys (LDS rows from kb on) and 16 dimensions (16 t on).
+template <int HD>
+__device__ __forceinline__ u32x4 k_fragment(const char* kb, int lane, int t)
 {
-    const char* row = kb + (lane & 31) * kRowK<HD> + (lane >> 5) * 16;
-    f32x16 s{};
-    #pragma unroll
-    for (int t = 0; t < HD / 16; ++t) s = mfma32<IO>(*(const u32x4*)(row + t * 32), qf[t], s);
-    return s;
+    return *(const u32x4*)(kb + (lane & 31) * kRowK<HD> + (lane >> 5) * 16 + t * 32);
 }
 
 // Which of the 32 keys from j0 on the lane's row sees: its scores elsewhere become -inf.
@@ -262,28 +258,16 @@ template <class IO> __device__ __forceinline__ float exponent_base(float m, floa
     return kShift<IO> - (m == -INFINITY ? 0.0f : m) * c;
 }
 
-// o^T += V^T P^T over 32 keys (LDS rows from vb on).  The probabilities are rounded to V's type for the matrix cores:
-// one rounding of at most half a step each, against the same reference for the whole row; l sums them unrounded.
-template <class IO, int HD>
-__device__ __forceinline__ void pv_tile(f32x16 (&o)[HD / 32], const f32x16& p, const char* vb, int lane)
+// V^T fragment of 16 keys (half u of the 32 at vb) and 32 columns (32 t on).
+template <int HD>
+__device__ __forceinline__ u32x4 v_fragment(const char* vb, int lane, int u, int t)
 {
     constexpr int RV = kRowV<HD, 32>;
     const char* r0 = vb + (4 * (lane >> 5) + ((lane >> 2) & 3)) * RV + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-    #pragma unroll
-    for (int u = 0; u < 2; ++u)
-    {
-        u32x4 pf;
-        #pragma unroll
-        for (int e = 0; e < 4; ++e) pf[e] = pack2<IO>(p[8 * u + 2 * e], p[8 * u + 2 * e + 1]);
-        #pragma unroll
-        for (int t = 0; t < HD / 32; ++t)
-        {
-            const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + u * 16 * RV + t * 64));
-            const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + (u * 16 + 8) * RV + t * 64));
-            const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
-            o[t] = mfma32<IO>(u32x4{ w0.x, w0.y, w1.x, w1.y }, pf, o[t]);
-        }
-    }
+    const auto v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + u * 16 * RV + t * 64));
+    const auto v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lptr<s16x4>)(r0 + (u * 16 + 8) * RV + t * 64));
+    const u32x2 w0 = __builtin_bit_cast(u32x2, v0), w1 = __builtin_bit_cast(u32x2, v1);
+    return u32x4{ w0.x, w0.y, w1.x, w1.y };
 }
 
 // Infinities and NaNs of V in a tile that some row does not see whole: there the probability is 0, but 0 * inf and
@@ -313,10 +297,10 @@ __device__ __forceinline__ void zero_nonfinite(u32x4& v)
         v[i] &= (nonfinite<IO>(v[i]) ? 0u : 0xffffu) | (nonfinite<IO>(v[i] >> 16) ? 0u : 0xffff0000u);
 }
 
-// The page of key j (-1 past the keys of the launch).
+// The page of key j, of the last key past the end.
 __device__ __forceinline__ int page_entry(const AttnArgs& a, const int32_t* table, int j, int khi)
 {
-    return j < khi ? table[j >> a.page_shift] : -1;
+    return ((gcptr<int32_t>)table)[min(j, khi - 1) >> a.page_shift];
 }
 
 // One tile's loads.  SMALL (pages of fewer keys than a tile): a lane's key has a page of its own, entry k of the
@@ -358,37 +342,40 @@ __device__ __forceinline__ void load_tile(const AttnArgs& a, int j0, int entry, 
     }
 }
 
-// A tile into LDS: keys that the launch must not see as zeros and, where not every row sees all of it (`part`),
-// without V's infinities and NaNs.  Returns whether there were such.
-template <class IO, int HD, int STEPS, int LANES, int RV>
-__device__ __forceinline__ bool write_tile(u32x4 (&ks)[STEPS], u32x4 (&vs)[STEPS], uint64_t ok, bool part, int lane_of_tile,
-                                           char* kl, char* vl)
+// A tile in registers of which not every row sees all: its keys that the launch must not see become zeros, V's infinities
+// and NaNs too.  Returns whether there were such.
+template <class IO, int HD, int STEPS, int LANES>
+__device__ __forceinline__ bool clean_tile(u32x4 (&ks)[STEPS], u32x4 (&vs)[STEPS], uint64_t ok, int lane_of_tile)
 {
     constexpr int CH = HD / 8, KPS = LANES / CH;
-    const int key = lane_of_tile / CH, ch = lane_of_tile % CH;
     bool odd = false;
-    if (part)
-    {
-        #pragma unroll
-        for (int k = 0; k < STEPS; ++k)
-        {
-            if (!((ok >> (k * KPS + key)) & 1)) ks[k] = vs[k] = u32x4{};
-            if (nonfinite8<IO>(vs[k]))
-            {
-                zero_nonfinite<IO>(vs[k]);
-                odd = true;
-            }
-        }
-    }
-    char* const kd = kl + key * kRowK<HD> + ch * 16;
-    char* const vd = vl + key * RV + ch * 16;
     #pragma unroll
     for (int k = 0; k < STEPS; ++k)
     {
-        *(u32x4*)(kd + k * KPS * kRowK<HD>) = ks[k];
-        *(u32x4*)(vd + k * KPS * RV) = vs[k];
+        if (!((ok >> (k * KPS + lane_of_tile / CH)) & 1)) ks[k] = vs[k] = u32x4{};
+        if (nonfinite8<IO>(vs[k]))
+        {
+            zero_nonfinite<IO>(vs[k]);
+            odd = true;
+        }
     }
     return odd;
+}
+
+// Step k of a tile in registers, or all of it, into LDS.
+template <int HD, int STEPS, int LANES, int RV>
+__device__ __forceinline__ void write_step(const u32x4 (&ks)[STEPS], const u32x4 (&vs)[STEPS], int k, int lane_of_tile, char* kl, char* vl)
+{
+    constexpr int CH = HD / 8, KPS = LANES / CH;
+    const int key = lane_of_tile / CH, ch = lane_of_tile % CH;
+    *(u32x4*)(kl + key * kRowK<HD> + ch * 16 + k * KPS * kRowK<HD>) = ks[k];
+    *(u32x4*)(vl + key * RV + ch * 16 + k * KPS * RV) = vs[k];
+}
+template <int HD, int STEPS, int LANES, int RV>
+__device__ __forceinline__ void write_tile(const u32x4 (&ks)[STEPS], const u32x4 (&vs)[STEPS], int lane_of_tile, char* kl, char* vl)
+{
+    #pragma unroll
+    for (int k = 0; k < STEPS; ++k) write_step<HD, STEPS, LANES, RV>(ks, vs, k, lane_of_tile, kl, vl);
 }
 
 // Calls add(j, v) for every key j of the tile at j0 with V's row there (global memory).
@@ -438,17 +425,21 @@ __device__ __forceinline__ void flag_positions(const AttnArgs& a, const QRow& r)
 }
 
 // ---------------------------------------------------------------------------------------------
-// Many query rows: WAVES waves of 32 rows each share tiles of KT keys in a ring of three LDS stages.  While a tile's
-// scores become probabilities (VALU), the matrix cores are at the next tile's scores; the tile after that is on its
-// way into the third stage, and the one after it in registers.  One barrier per tile.
+// Many query rows: WAVES waves of 32 rows each share tiles of KT keys in a ring of three LDS stages.  A wave's step is a
+// slot of products (o += V(i) P(i), then the scores of tile i + 1) and a slot of softmax (those scores to P(i + 1), and
+// its part of a later tile's loads and LDS writes), with a barrier after each.  Of 8 waves, 4 .. 7 (the second wave of
+// each SIMD) run one slot behind 0 .. 3, so that one wave of a SIMD is at the matrix cores while the other is at the
+// VALU: in step, both wait for the same unit.
 template <class IO, int HD, int WAVES, int KT, bool SMALL>
 __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
 {
     constexpr int LANES = WAVES * 64, RK = kRowK<HD>, RV = kRowV<HD, 32>, STEPS = KT * (HD / 8) / LANES, NS = KT / 32;
     constexpr int STAGE = KT * (RK + RV);
+    constexpr uint64_t FULL = KT == 64 ? ~0ull : 0xffffffffull;
     __shared__ __align__(16) char lds[3 * STAGE];
     __shared__ int plo[WAVES], phi[WAVES], odd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const int late = WAVES == 8 ? wave >> 2 : 0;
     const Item it = launch_item(a);
     const int r0 = it.tile * (32 * WAVES) + wave * 32;
     const QRow row = query_row(a, it.set, it.kvh, min(r0 + (lane & 31), a.rows - 1));
@@ -474,63 +465,23 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
     #pragma unroll
     for (int t = 0; t < HD / 32; ++t) o[t] = f32x16{};
     float m = -INFINITY, l = 0.0f;
-
-    u32x4 ks[STEPS], vs[STEPS];
-    int entry = -1;
-    uint64_t ok_load = 0;      // of the tile in registers
-    const auto fetch_entry = [&](int i) { entry = i < t1 ? page_entry(a, table, tile_key(i) + (lane & (KT - 1)), tl.khi) : -1; };
-    const auto load = [&](int i) {
-        if (i >= t1) return;
-        const int j0 = tile_key(i);
-        const bool in = key_seen(a, tl, j0 + (lane & (KT - 1)), gmin), good = in && (uint64_t)(int64_t)entry < (uint64_t)a.num_pages;
-        if (a.err && in && !good) *a.err = 1;
-        ok_load = __ballot(good);
-        if (KT == 32) ok_load &= 0xffffffffu;
-        load_tile<HD, SMALL, STEPS, LANES>(a, j0, entry, ok_load, it.kvh, tid, ks, vs);
-        fetch_entry(i + 1);
-    };
-    constexpr uint64_t FULL = KT == 64 ? ~0ull : 0xffffffffull;
-    const auto write = [&](int i) {      // the tile in registers into its stage
-        if (i >= t1) return;
-        char* const st = lds + ((i - t0) % 3) * STAGE;
-        const bool part = ok_load != FULL || !all_seen(a, tile_key(i), KT, gmin, gmax);
-        if (write_tile<IO, HD, STEPS, LANES, RV>(ks, vs, ok_load, part, tid, st, st + KT * RK)) odd = 1;
-    };
-    uint64_t ok_now = 0, ok_next = 0;    // of tiles i and i + 1
-    fetch_entry(t0);
-    load(t0);
-    write(t0);
-    ok_now = ok_load;
-    load(t0 + 1);
-    __syncthreads();
-    f32x16 sa[NS], sb[NS];
-    const auto scores = [&](int i, f32x16 (&s)[NS]) {
-        const char* const st = lds + ((i - t0) % 3) * STAGE;
-        #pragma unroll
-        for (int k = 0; k < NS; ++k) s[k] = qk_tile<IO, HD>(st + k * 32 * RK, lane, qf);
-    };
-    if (t0 < t1) scores(t0, sa);
-    write(t0 + 1);
-    ok_next = ok_load;
-    load(t0 + 2);
-    __syncthreads();
     const float slack = kSlack / a.c;
-    // Tile i, whose scores are in s; the next tile's go to sn.
-    const auto step = [&](int i, f32x16 (&s)[NS], f32x16 (&sn)[NS]) __attribute__((always_inline)) {
-        const int j0 = tile_key(i);
-        const char* const st = lds + ((i - t0) % 3) * STAGE;
-        if (ok_now != FULL || !all_seen(a, j0, KT, pmin, pmax))
+    f32x16 s[NS];
+    u32x4 pf[2 * NS];       // P of 16 keys each
+    const auto softmax = [&](int i, uint64_t ok, bool part) {
+        if (part)
         {
+            const int j0 = tile_key(i);
             #pragma unroll
             for (int k = 0; k < NS; ++k)
-                mask_tile(s[k], j0 + 32 * k, half, row.p, a.window, a.sinks, (uint32_t)(ok_now >> (32 * k)));
+                mask_tile(s[k], j0 + 32 * k, half, row.p, a.window, a.sinks, (uint32_t)(ok >> (32 * k)));
         }
-        float mx = s[0][0];
+        float mx4[4] = { s[0][0], s[0][1], s[0][2], s[0][3] };
         #pragma unroll
         for (int k = 0; k < NS; ++k)
             #pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][e]);
-        mx = max_xor32(mx);
+            for (int e = k ? 0 : 4; e < 16; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], s[k][e]);
+        const float mx = max_xor32(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
         if (__any(mx > m + slack))
         {
             const float mn = fmaxf(m, mx), alpha = rescale_factor(m, mn, a.c);
@@ -541,31 +492,161 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
                 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
         }
-        scores(i + 1, sn);
         const float base = exponent_base<IO>(m, a.c);
         float sum[4] = {};
         #pragma unroll
         for (int k = 0; k < NS; ++k)
+        {
             #pragma unroll
             for (int e = 0; e < 16; ++e)
             {
                 s[k][e] = __builtin_amdgcn_exp2f(fmaf(s[k][e], a.c, base));
                 sum[e & 3] += s[k][e];
             }
+            #pragma unroll
+            for (int e = 0; e < 8; ++e) pf[2 * k + e / 4][e % 4] = pack2<IO>(s[k][2 * e], s[k][2 * e + 1]);
+        }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        #pragma unroll
-        for (int k = 0; k < NS; ++k) pv_tile<IO, HD>(o, s[k], st + KT * RK + k * 32 * RV, lane);
-        write(i + 2);
-        ok_now = ok_next;
-        ok_next = ok_load;
-        load(i + 3);
-        __syncthreads();
     };
-    for (int i = t0; i < t1; i += 2)
+
+    if (t0 < t1)
     {
-        step(i, sa, sb);
-        if (i + 1 < t1) step(i + 1, sb, sa);
+        // The tiles of the list that every row of the workgroup, or of the wave, sees whole: [f0, gf1) and [f0 or its own,
+        // wf1) (the sinks' tiles aside).
+        const auto whole_from = [&](int pmx) { return a.window > 0 ? max(tl.ns, tl.ns - tl.wt + (max(max(pmx - a.window + 1, 0) - a.dom_lo, 0) + KT - 1) / KT) : tl.ns; };
+        const auto whole_to = [&](int pmn) { return tl.ns - tl.wt + max(min(pmn, 0x7ffffffe) + 1 - a.dom_lo, 0) / KT; };
+        const int gf0 = whole_from(gmax), gf1 = whole_to(gmin), wf0 = whole_from(pmax), wf1 = whole_to(pmin);
+
+        // Loads.  SMALL: every key's page is looked up.  Otherwise a tile lies in one page and follows the one before it,
+        // but for the step from the sinks to the window; `off` is its first row's byte offset for this KV head.  Past the
+        // last tile the last one is loaded again.
+        u32x4 ks[STEPS], vs[STEPS];
+        const uint32_t row_bytes = (uint32_t)a.hk * (HD * 2);
+        const int in_page = (1 << a.page_shift) - 1, last_page = (tl.khi - 1) >> a.page_shift;
+        uint64_t ok0 = 0, ok1 = 0, ok2 = 0;      // the visible keys of the last three tiles loaded that have a page
+        bool bad = false;
+        int entry = 0, ahead = 0, il = t0;       // (SMALL: a key's page each) page of tile il, of the page after it
+        int64_t off = 0;
+        const auto enter_page = [&](int j, int e) {      // tile il starts at key j of page e
+            const bool good = (uint32_t)e < (uint32_t)a.num_pages;
+            bad |= !good;
+            entry = good;
+            off = ((int64_t)(good ? e : 0) << a.page_shift) + (j & in_page);
+            off = off * row_bytes + it.kvh * (HD * 2);
+            ahead = ((gcptr<int32_t>)table)[min((j >> a.page_shift) + 1, last_page)];
+        };
+        if constexpr (SMALL) entry = page_entry(a, table, tile_key(t0) + (lane & (KT - 1)), tl.khi);
+        else enter_page(tile_key(t0), __builtin_amdgcn_readfirstlane(((gcptr<int32_t>)table)[tile_key(t0) >> a.page_shift]));
+        const uint32_t lane_off = tid / (HD / 8) * row_bytes + tid % (HD / 8) * 16;
+        const auto load = [&]() {
+            ok2 = ok1;
+            ok1 = ok0;
+            if constexpr (SMALL)
+            {
+                const int j0 = tile_key(il);
+                const bool in = key_seen(a, tl, j0 + (lane & (KT - 1)), gmin), good = in && (uint32_t)entry < (uint32_t)a.num_pages;
+                bad |= in && !good;
+                ok0 = __ballot(good) & FULL;
+                load_tile<HD, SMALL, STEPS, LANES>(a, j0, entry, ok0, it.kvh, tid, ks, vs);
+                if (il + 1 < t1) ++il;
+                entry = page_entry(a, table, tile_key(il) + (lane & (KT - 1)), tl.khi);
+            }
+            else
+            {
+                ok0 = entry ? FULL : 0;
+                const char *kb = a.kc + off, *vb = a.vc + off;
+                #pragma unroll
+                for (int k = 0; k < STEPS; ++k)
+                {
+                    ks[k] = *(gcptr<u32x4>)(kb + lane_off);
+                    vs[k] = *(gcptr<u32x4>)(vb + lane_off);
+                    kb += LANES / (HD / 8) * row_bytes;
+                    vb += LANES / (HD / 8) * row_bytes;
+                }
+                if (il + 1 < t1)
+                {
+                    ++il;
+                    const int j = tile_key(il);
+                    if (il == tl.ns) enter_page(j, __builtin_amdgcn_readfirstlane(((gcptr<int32_t>)table)[j >> a.page_shift]));
+                    else if ((j & in_page) == 0) enter_page(j, __builtin_amdgcn_readfirstlane(ahead));
+                    else off += KT * row_bytes;
+                }
+            }
+        };
+        // The tile loaded last, tile i, into stage st: clean where not every row sees all of it.
+        const auto write = [&](int i, char* st) {
+            i = min(i, t1 - 1);
+            if (i < gf0 || i >= gf1 || ok0 != FULL)
+            {
+                uint64_t seen = ok0;
+                if (!SMALL) seen &= __ballot(key_seen(a, tl, tile_key(i) + (lane & (KT - 1)), gmin));
+                if (clean_tile<IO, HD, STEPS, LANES>(ks, vs, seen, tid)) odd = 1;
+            }
+            write_tile<HD, STEPS, LANES, RV>(ks, vs, tid, st, st + KT * RK);
+        };
+
+        // A slot's products: o += V P with V of stage v (if `step`), then the scores of the keys of stage k.  LDS reads run
+        // 8 MFMAs ahead of their use, in this order exactly: left to itself the compiler reads just before it
+        // multiplies, and waits for each read.
+        const auto products = [&](auto step, const char* v, const char* k) __attribute__((always_inline)) {
+            constexpr int N = NS * HD / 16, AHEAD = 8;      // MFMAs of each product
+            constexpr int from = decltype(step)::value ? 0 : N;
+            u32x4 f[AHEAD];
+            const auto read = [&](int j) {
+                if (j < N) f[j % AHEAD] = v_fragment<HD>(v + KT * RK + j / (HD / 16) * 32 * RV, lane, j / (HD / 32) % 2, j % (HD / 32));
+                else f[j % AHEAD] = k_fragment<HD>(k + (j - N) % NS * 32 * RK, lane, (j - N) / NS);
+            };
+            #pragma unroll
+            for (int j = 0; j < AHEAD; ++j) read(from + j);
+            #pragma unroll
+            for (int j = from; j < 2 * N; ++j)
+            {
+                __builtin_amdgcn_sched_barrier(0);
+                if (j < N) o[j % (HD / 32)] = mfma32<IO>(f[j % AHEAD], pf[j / (HD / 32)], o[j % (HD / 32)]);
+                else s[(j - N) % NS] = mfma32<IO>(f[j % AHEAD], qf[(j - N) / NS], j - N < NS ? f32x16{} : s[(j - N) % NS]);
+                if (j + AHEAD < 2 * N) read(j + AHEAD);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const auto probabilities = [&](int i, uint64_t ok) { softmax(i, ok, i < wf0 || i >= wf1 || ok != FULL); };
+
+        // The stages of tiles i, i + 1 and i + 2.  The late waves write, and load, a tile further: tile i + 3's stage held
+        // tile i, which they are the last to read.
+        char *sa = lds, *sb = lds + STAGE, *sc = lds + 2 * STAGE;
+        load();
+        write(t0, sa);
+        load();
+        write(t0 + 1, sb);
+        load();
+        const uint64_t first = ok2;
+        if (late)
+        {
+            write(t0 + 2, sc);
+            load();
+        }
+        __syncthreads();
+        if (late) __syncthreads();
+        products(std::false_type{}, sa, sa);
+        __syncthreads();
+        probabilities(t0, first);
+        __syncthreads();
+        for (int i = t0; i < t1; ++i)
+        {
+            products(std::true_type{}, sa, sb);
+            __syncthreads();
+            if (i + 1 < t1) probabilities(i + 1, late ? ok2 : ok1);
+            write(i + 2 + late, late ? sa : sc);
+            load();
+            char* const st = sa;
+            sa = sb;
+            sb = sc;
+            sc = st;
+            __syncthreads();
+        }
+        if (!late && WAVES == 8) __syncthreads();
+        if (a.err && bad) *a.err = 1;
     }
+    __syncthreads();
     if (odd)
         for (int i = t0; i < t1; ++i)
             each_value_row<HD>(a, tl, table, tile_key(i), KT, it.kvh, [&](int j, gcptr<uint16_t> v) {
@@ -644,7 +725,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
     int entry = -1;
     uint32_t ok_next = 0;
     auto fetch_entry = [&](int i) {
-        entry = i < t1 ? page_entry(a, table, a.dom_lo + tl.tile(i) * KT + (lane & 31), tl.khi) : -1;
+        if (i < t1) entry = page_entry(a, table, a.dom_lo + tl.tile(i) * KT + (lane & 31), tl.khi);
     };
     auto stage = [&](int i) {
         const int j0 = a.dom_lo + tl.tile(i) * KT;
@@ -679,7 +760,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         const int j = a.dom_lo + tl.tile(i) * KT;
         const bool whole = ok == 0xffffffffu && all_seen(a, j, KT, pmin, pmax);
         wave_lds_fence();
-        odd |= write_tile<IO, HD, STEPS, 64, RV>(ks, vs, ok, !whole, lane, kl, vl);
+        if (!whole) odd |= clean_tile<IO, HD, STEPS, 64>(ks, vs, ok, lane);
+        write_tile<HD, STEPS, 64, RV>(ks, vs, lane, kl, vl);
         wave_lds_fence();
         if (i + 4 < t1) { stage(i + 4); fetch_entry(i + 8); }
         if (ok == 0) continue;
