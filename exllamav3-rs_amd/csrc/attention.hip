@@ -13,6 +13,7 @@
 // transposing LDS read (ds_read_b64_tr_b16) delivers: 4 consecutive keys of one column per read.
 // A query row of the kernels is a (token, query head) pair: the heads that share a KV head are packed together,
 // so one read of K and V serves the whole group.
+#include <algorithm>
 #include "abi.hpp"
 #include "common.cuh"
 
@@ -24,7 +25,20 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 template <class T> using lptr = __attribute__((address_space(3))) T*;
 
-constexpr int kMaxSplits = 512;      // of a row: 256 of the shared prefix and 256 of its own keys
+constexpr int kMaxSplits = 512;      // of a row in one launch
+
+// Where a launch leaves the partial results of its rows: o unnormalised, {c m - shift, l}, fp32.  Partial i of a row:
+//   k_attn_rows: of `n` fixed splits, at [global row][i];
+//   k_attn_keys (`info` set): of the workgroups ("slots") info[seg].x .. info[seg].y that share its segment, at
+//   [KV head][slot + seg][row of the segment]: slot + seg never meets itself, as walking the slots one or the other
+//   grows.
+struct Parts
+{
+    float* po;
+    float* ml;
+    int32_t* info;
+    int32_t n, slots, segs, row_tiles, seg_rows, whole;
+};
 
 struct AttnArgs
 {
@@ -36,8 +50,7 @@ struct AttnArgs
     const int32_t* table;
     const int32_t* lens;
     int32_t* err;
-    float* po;                // partial outputs [row][split][HD], unnormalised
-    float* pml;               // ... and their {c m - shift, l} [row][split][2]
+    Parts parts;              // of this launch
     int64_t q_ts, q_hs, o_ts, o_hs;     // elements
     int64_t max_blocks, num_pages;
     int64_t rows_all;         // bsz * seq * hq
@@ -45,9 +58,9 @@ struct AttnArgs
     int32_t page_shift, window, sinks;
     int32_t dom_lo, dom_hi;   // keys of this launch: [dom_lo, dom_hi)
     int32_t rows;             // query rows per row set (a sequence's, or the whole batch's)
-    int32_t row_tiles, nsplit, split0, splits;   // this launch's splits, their first place among all `splits`
+    int32_t row_tiles;
     int32_t whole;            // 1: one row set of all sequences, keys through sequence 0's table row
-    int32_t direct;           // 1: this launch's result is the output
+    int32_t direct;           // 1: a result that no other split shares is the output
     int32_t q_vec, o_vec;     // 16-byte aligned q rows / 8-byte aligned out rows
     float c;
 };
@@ -147,6 +160,12 @@ __device__ __forceinline__ int wave_max(int v)
     #pragma unroll
     for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d));
     return __builtin_amdgcn_readfirstlane(v);
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t v)
+{
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
 __device__ __forceinline__ float max_wave(float v)
@@ -311,11 +330,13 @@ __device__ __forceinline__ void load_tile(const AttnArgs& a, int j0, int entry, 
                                           u32x4 (&ks)[STEPS], u32x4 (&vs)[STEPS])
 {
     constexpr int CH = HD / 8, KPS = LANES / CH;      // keys per step
-    const int key0 = lane_of_tile / CH, ch = lane_of_tile % CH;
+    int key0 = lane_of_tile / CH, ch = lane_of_tile % CH;
     const uint32_t row_bytes = (uint32_t)a.hk * (HD * 2);
     const int in_page = (1 << a.page_shift) - 1;
     if constexpr (SMALL)
     {
+        // (decode: the steps' addresses are not kept in registers from tile to tile)
+        if constexpr (LANES == 64) asm volatile("" : "+v"(key0), "+v"(ch));
         #pragma unroll
         for (int k = 0; k < STEPS; ++k)
         {
@@ -413,15 +434,15 @@ __device__ __forceinline__ Item launch_item(const AttnArgs& a)
     x /= (uint32_t)a.hk;
     it.tile = a.row_tiles - 1 - (int)(x % (uint32_t)a.row_tiles);
     x /= (uint32_t)a.row_tiles;
-    it.split = x % (uint32_t)a.nsplit;
-    it.set = x / (uint32_t)a.nsplit;
+    it.split = x % (uint32_t)a.parts.n;
+    it.set = x / (uint32_t)a.parts.n;
     return it;
 }
 
-__device__ __forceinline__ void flag_positions(const AttnArgs& a, const QRow& r)
+__device__ __forceinline__ void flag_positions(const AttnArgs& a, int p)
 {
     const int64_t cap = a.max_blocks << a.page_shift;
-    if (a.err && (r.p < 0 || r.p >= cap)) *a.err = 1;
+    if (a.err && (p < 0 || p >= cap)) *a.err = 1;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -431,7 +452,7 @@ __device__ __forceinline__ void flag_positions(const AttnArgs& a, const QRow& r)
 // each SIMD) run one slot behind 0 .. 3, so that one wave of a SIMD is at the matrix cores while the other is at the
 // VALU: in step, both wait for the same unit.
 template <class IO, int HD, int WAVES, int KT, bool SMALL>
-__global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
+__global__ __launch_bounds__(WAVES * 64, HD == 256 ? 1 : 2) void k_attn_rows(AttnArgs a)
 {
     constexpr int LANES = WAVES * 64, RK = kRowK<HD>, RV = kRowV<HD, 32>, STEPS = KT * (HD / 8) / LANES, NS = KT / 32;
     constexpr int STAGE = KT * (RK + RV);
@@ -443,7 +464,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
     const Item it = launch_item(a);
     const int r0 = it.tile * (32 * WAVES) + wave * 32;
     const QRow row = query_row(a, it.set, it.kvh, min(r0 + (lane & 31), a.rows - 1));
-    if (it.split == 0 && it.kvh == 0) flag_positions(a, row);
+    if (it.split == 0 && it.kvh == 0) flag_positions(a, row.p);
     const int pmin = wave_min(row.p), pmax = wave_max(row.p);
     if (lane == 0) { plo[wave] = pmin; phi[wave] = pmax; }
     if (tid == 0) odd = 0;
@@ -456,7 +477,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
     gmin = __builtin_amdgcn_readfirstlane(gmin);
     gmax = __builtin_amdgcn_readfirstlane(gmax);
     const TileList tl = tile_list(a, gmin, gmax, KT);
-    const int per = (tl.count + a.nsplit - 1) / a.nsplit;
+    const int per = (tl.count + a.parts.n - 1) / a.parts.n;
     const int t0 = min(it.split * per, tl.count), t1 = min(t0 + per, tl.count);
     const int32_t* table = a.table + (a.whole ? 0 : (int64_t)it.set * a.max_blocks);
     const auto tile_key = [&](int i) { return a.dom_lo + tl.tile(i) * KT; };
@@ -675,10 +696,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
     }
     else
     {
-        const int64_t pr = gr * a.splits + a.split0 + it.split;
-        if (half == 0) { a.pml[2 * pr] = fmaf(m, a.c, -kShift<IO>); a.pml[2 * pr + 1] = l; }
+        const int64_t pr = gr * a.parts.n + it.split;
+        if (half == 0) { a.parts.ml[2 * pr] = fmaf(m, a.c, -kShift<IO>); a.parts.ml[2 * pr + 1] = l; }
         if (l == 0.0f) return;
-        gptr<f32x4> d = (gptr<f32x4>)(a.po + pr * HD + 4 * half);
+        gptr<f32x4> d = (gptr<f32x4>)(a.parts.po + pr * HD + 4 * half);
         #pragma unroll
         for (int t = 0; t < HD / 32; ++t)
             #pragma unroll
@@ -693,34 +714,134 @@ __global__ __launch_bounds__(WAVES * 64, WAVES / 4) void k_attn_rows(AttnArgs a)
 // column tile (v_mfma_f32_16x16x32: lane l holds row l % 16, keys 4 (l / 16) + i of each 16) a group of 8 or 16 query
 // heads leaves little of a tile empty, and o, Q and the scores take half the registers of 32 rows, so that two tiles
 // of loads per SIMD stay in flight: HBM is the bound here.
+// The work is cut by keys, not by rows: the row tiles of all sequences ("segments"), in units of 128 keys, make one
+// list per KV head, and each of `slots` workgroups takes an equal part of it, whatever the lengths.  Every workgroup
+// counts the units itself, from cache_seqlens; a segment that one slot has whole goes straight to the output.
+
+// The units of segment g (never 0: its rows are written also where they see nothing).
+__device__ __forceinline__ int list_units(const TileList& l) { return max(1, (l.count + 3) / 4); }
+
+__device__ __forceinline__ int segment_units(const AttnArgs& a, int g)
+{
+    const int b = g / a.row_tiles, r0 = (g - b * a.row_tiles) * a.parts.seg_rows, r1 = min(r0 + a.parts.seg_rows, a.rows) - 1;
+    const int64_t len = a.lens[b], lo = len + r0 / a.group, hi = len + r1 / a.group;
+    return list_units(tile_list(a, (int)min(max(lo, (int64_t)-1), (int64_t)0x7fffffff),
+                                (int)min(max(hi, (int64_t)-1), (int64_t)0x7fffffff), 32));
+}
+
 template <class IO, int HD, int NC, bool SMALL>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a)
 {
     constexpr int KT = 32, RK = kRowK<HD>, RV = kRowV<HD, 16>, STEPS = KT * (HD / 8) / 64, ROWS = 16 * NC;
     __shared__ __align__(16) char lds[4][KT * (RK + RV)];
     __shared__ float mlw[4][2][ROWS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4, col = lane & 15;
+    __shared__ int64_t sums[4], begin[2];
+    int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     char* const kl = lds[wave];
     char* const vl = lds[wave] + KT * RK;
-    const Item it = launch_item(a);
-    const int r0 = it.tile * ROWS;
-    QRow row[NC];
-    int pmin = 0x7fffffff, pmax = -0x7fffffff;
-    #pragma unroll
-    for (int n = 0; n < NC; ++n)
-    {
-        row[n] = query_row(a, it.set, it.kvh, min(r0 + 16 * n + col, a.rows - 1));
-        if (it.split == 0 && it.kvh == 0) flag_positions(a, row[n]);
-        pmin = min(pmin, row[n].p);
-        pmax = max(pmax, row[n].p);
-    }
-    pmin = wave_min(pmin);
-    pmax = wave_max(pmax);
-    const TileList tl = tile_list(a, pmin, pmax, KT);
-    const int per = ((tl.count + a.nsplit - 1) / a.nsplit + 3) & ~3;
-    const int t0 = min(it.split * per, tl.count), t1 = min(t0 + per, tl.count);
+    const int kvh = blockIdx.x % (uint32_t)a.hk, slot = blockIdx.x / (uint32_t)a.hk, segs = a.parts.segs;
 
-    const int32_t* table = a.table + (a.whole ? 0 : (int64_t)it.set * a.max_blocks);
+    int pos[NC], set = 0, r0 = 0, pmin = 0, pmax = 0, units = 0;
+    TileList tl{};
+    const auto enter = [&](int g) {
+        const int col = tid & 15;
+        set = a.whole ? 0 : g / a.row_tiles;
+        r0 = (g - set * a.row_tiles) * ROWS;
+        pmin = 0x7fffffff;
+        pmax = -0x7fffffff;
+        #pragma unroll
+        for (int n = 0; n < NC; ++n)
+        {
+            pos[n] = query_row(a, set, kvh, min(r0 + 16 * n + col, a.rows - 1)).p;
+            pmin = min(pmin, pos[n]);
+            pmax = max(pmax, pos[n]);
+        }
+        pmin = wave_min(pmin);
+        pmax = wave_max(pmax);
+        tl = tile_list(a, pmin, pmax, KT);
+        units = list_units(tl);
+    };
+    // The slot's units [x0, x1), the segment that x0 lies in and that segment's first unit.
+    int64_t total = 0, start = 0;
+    int g = 0;
+    if (segs == 1)
+    {
+        enter(0);
+        total = units;
+    }
+    else
+    {
+        const int each = (segs + 255) / 256, g0 = min(tid * each, segs), g1 = min(g0 + each, segs);
+        int64_t mine = 0;
+        if (!a.whole)
+            for (int i = g0; i < g1; ++i) mine += segment_units(a, i);
+        else        // (two row tiles at most)
+            for (int i = 0; i < segs; ++i)
+            {
+                enter(i);
+                if (g0 <= i && i < g1) mine += units;
+            }
+        int64_t before = mine;
+        #pragma unroll
+        for (int d = 1; d < 64; d <<= 1)
+        {
+            const int64_t v = __shfl_up(before, d);
+            if ((tid & 63) >= d) before += v;
+        }
+        if ((tid & 63) == 63) sums[wave] = before;
+        __syncthreads();
+        before -= mine;
+        #pragma unroll
+        for (int w = 0; w < 4; ++w)
+        {
+            if (w < wave) before += sums[w];
+            total += sums[w];
+        }
+        const int64_t x = slot * ((total + a.parts.slots - 1) / a.parts.slots);
+        if (x >= before && x < before + mine)
+        {
+            if (!a.whole)
+                for (g = g0; ; ++g)
+                {
+                    const int u = segment_units(a, g);
+                    if (x < before + u) break;
+                    before += u;
+                }
+            else g = g0;        // (one segment per lane)
+            begin[0] = g;
+            begin[1] = before;
+        }
+        __syncthreads();
+        g = __builtin_amdgcn_readfirstlane((int)begin[0]);
+        start = uniform64(begin[1]);
+        total = uniform64(total);
+    }
+    const int64_t share = uniform64((total + a.parts.slots - 1) / a.parts.slots), x0 = slot * share, x1 = min(x0 + share, total);
+    if (x0 >= total) return;
+    const float slack = kSlack / a.c;
+    for (;; ++g)
+    {
+    if (segs != 1) enter(g);
+    // (Pinned here and below: what a lane computes from its number would be kept across the loop over the segments, in
+    // registers that the loop over the keys needs.)
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, quad = lane >> 4, col = lane & 15;
+    const int u0 = (int)max(x0 - start, (int64_t)0), u1 = (int)min(x1 - start, (int64_t)units);
+    const int t0 = __builtin_amdgcn_readfirstlane(min(4 * u0, tl.count)), t1 = __builtin_amdgcn_readfirstlane(min(4 * u1, tl.count));
+    if (u0 == 0 && kvh == 0)
+    {
+        #pragma unroll
+        for (int n = 0; n < NC; ++n) flag_positions(a, pos[n]);
+        if (tid == 0 && a.parts.info)
+        {
+            a.parts.info[2 * g] = slot;
+            a.parts.info[2 * g + 1] = (int)((start + units - 1) / share);
+        }
+    }
+    const bool direct = a.direct && u0 == 0 && u1 == units;
+
+    const int32_t* table = a.table + (a.whole ? 0 : (int64_t)set * a.max_blocks);
     u32x4 ks[STEPS], vs[STEPS];
     int entry = -1;
     uint32_t ok_next = 0;
@@ -732,7 +853,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         const bool in = key_seen(a, tl, j0 + (lane & 31), pmin), good = in && (uint64_t)(int64_t)entry < (uint64_t)a.num_pages;
         if (a.err && in && !good) *a.err = 1;
         ok_next = (uint32_t)__ballot(good);
-        load_tile<HD, SMALL, STEPS, 64>(a, j0, entry, ok_next, it.kvh, lane, ks, vs);
+        load_tile<HD, SMALL, STEPS, 64>(a, j0, entry, ok_next, kvh, lane, ks, vs);
     };
     fetch_entry(t0 + wave);
     if (t0 + wave < t1) { stage(t0 + wave); fetch_entry(t0 + wave + 4); }
@@ -743,7 +864,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
     #pragma unroll
     for (int n = 0; n < NC; ++n)
     {
-        load_q<IO, HD, 32>(a, row[n], quad, qf[n]);
+        load_q<IO, HD, 32>(a, query_row(a, set, kvh, min(r0 + 16 * n + col, a.rows - 1)), quad, qf[n]);
         #pragma unroll
         for (int t = 0; t < HD / 16; ++t) o[n][t] = f32x4{};
         m[n] = -INFINITY;
@@ -752,7 +873,6 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
     // K fragment: key row col (of 16), chunks 4 t + quad; V^T fragment: keys 4 quad + 0..3 (and + 16), columns 16 t + col
     const char* const krow = kl + col * RK + quad * 16;
     const char* const vrow = vl + (4 * quad + (col >> 2)) * RV + (col & 3) * 8;
-    const float slack = kSlack / a.c;
     bool odd = false;
     for (int i = t0 + wave; i < t1; i += 4)
     {
@@ -785,7 +905,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         {
             if (!whole)
             {
-                const int p = row[n].p, lo = a.window > 0 ? p - a.window + 1 : 0;
+                const int p = pos[n], lo = a.window > 0 ? p - a.window + 1 : 0;
                 const uint32_t okq = ok >> (4 * quad);
                 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -836,7 +956,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
     }
     if (__any(odd))
         for (int i = t0 + wave; i < t1; i += 4)
-            each_value_row<HD>(a, tl, table, a.dom_lo + tl.tile(i) * KT, KT, it.kvh, [&](int j, gcptr<uint16_t> v) {
+            each_value_row<HD>(a, tl, table, a.dom_lo + tl.tile(i) * KT, KT, kvh, [&](int j, gcptr<uint16_t> v) {
                 #pragma unroll
                 for (int t = 0; t < HD / 16; ++t)
                     #pragma unroll
@@ -846,7 +966,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
                         if (!nonfinite<IO>(h)) continue;
                         #pragma unroll
                         for (int n = 0; n < NC; ++n)
-                            if (row_sees(a, row[n].p, j)) o[n][t][e] += load_bits<IO>(h);
+                            if (row_sees(a, pos[n], j)) o[n][t][e] += load_bits<IO>(h);
                     }
             });
     // Join the waves: o against the common maximum, through LDS as [row][HD] floats with the 16-byte chunks of a
@@ -879,6 +999,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         }
     }
     __syncthreads();
+    asm volatile("" : "+v"(tid));
     // 256 lanes walk the rows: HD / 4 lanes of four columns each per row.
     constexpr int LPR = HD / 4, RPS = 256 / LPR;
     const int nr = min(ROWS, a.rows - r0);
@@ -898,9 +1019,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         const float rf = (mm == -INFINITY ? 0.0f : mm) * a.c;
         #pragma unroll
         for (int w = 0; w < 4; ++w) ls = fmaf(mlw[w][1][r], __builtin_amdgcn_exp2f(fmaf(mlw[w][0][r], a.c, -rf)), ls);
-        const QRow qr = query_row(a, it.set, it.kvh, r0 + r);
+        const QRow qr = query_row(a, set, kvh, r0 + r);
         const int64_t gr = qr.tok * a.hq + qr.h;
-        if (a.direct)
+        if (direct)
         {
             const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
             if (a.lse && ch == 0) a.lse[gr] = ls == 0.0f ? -INFINITY : (rf - kShift<IO> + __builtin_amdgcn_logf(ls)) * kLn2;
@@ -908,56 +1029,98 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
         }
         else
         {
-            const int64_t pr = gr * a.splits + a.split0 + it.split;
-            if (ch == 0) { a.pml[2 * pr] = fmaf(mm, a.c, -kShift<IO>); a.pml[2 * pr + 1] = ls; }
-            if (ls != 0.0f) ((gptr<f32x4>)(a.po + pr * HD))[ch] = sum;
+            const int64_t pr = ((int64_t)kvh * (a.parts.slots + segs) + slot + g) * a.parts.seg_rows + r;
+            if (ch == 0) { a.parts.ml[2 * pr] = fmaf(mm, a.c, -kShift<IO>); a.parts.ml[2 * pr + 1] = ls; }
+            if (ls != 0.0f) ((gptr<f32x4>)(a.parts.po + pr * HD))[ch] = sum;
         }
+    }
+    start += units;
+    if (start >= x1) break;
+    __syncthreads();        // the next segment's tiles overwrite what was joined
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Joins the splits of a row: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  WAVES waves per row; a wave takes
-// 256 / HD splits at a time (HD / 4 lanes of four columns each).
+// Joins the partial results of a row: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  WAVES waves per row; a wave
+// takes 256 / HD partial rows at a time (HD / 4 lanes of four columns each).
+struct JoinArgs
+{
+    Parts p[2];       // of the shared prefix (n 0 and no info: none), of the own keys
+};
+
+// A row's partial results of one launch: the first one's index, how many, the step between them.
+struct PartList
+{
+    int64_t at, step;
+    int n;
+};
+
+__device__ __forceinline__ PartList part_list(const AttnArgs& a, const Parts& p, int64_t gr, int b, int t, int h)
+{
+    PartList l{ gr * p.n, 1, p.n };
+    if (p.info)
+    {
+        const int kvh = h / a.group, r = (p.whole ? b * a.seq + t : t) * a.group + (h - kvh * a.group), tile = r / p.seg_rows;
+        const int seg = (p.whole ? 0 : b * p.row_tiles) + tile;
+        const int first = p.info[2 * seg], last = p.info[2 * seg + 1];
+        l.at = ((int64_t)kvh * (p.slots + p.segs) + first + seg) * p.seg_rows + (r - tile * p.seg_rows);
+        l.step = p.seg_rows;
+        l.n = last - first + 1;
+    }
+    return l;
+}
+
 template <class IO, int HD, int WAVES>
-__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a)
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a, JoinArgs j)
 {
     constexpr int LPR = HD / 4, SPW = 64 / LPR;       // lanes per partial row, partial rows per wave
-    __shared__ float wt[4 / WAVES][kMaxSplits];
+    __shared__ float wt[4 / WAVES][2 * kMaxSplits];
     __shared__ f32x4 part[4][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, local = wave / WAVES, sub = wave % WAVES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), local = wave / WAVES, sub = wave % WAVES;
     const int64_t gr = min((int64_t)blockIdx.x * (4 / WAVES) + local, a.rows_all - 1);
-    const int ns = a.splits;
-    const gcptr<f32x2> ml = (gcptr<f32x2>)(a.pml + 2 * gr * ns);
+    const int tok = (int)(gr / a.hq), h = (int)(gr - (int64_t)tok * a.hq), b = tok / a.seq;
+    const PartList pre = part_list(a, j.p[0], gr, b, tok - b * a.seq, h), own = part_list(a, j.p[1], gr, b, tok - b * a.seq, h);
+    const int n0 = __builtin_amdgcn_readfirstlane(pre.n), ns = n0 + __builtin_amdgcn_readfirstlane(own.n);
+    // A row that one slot had whole is written already.
+    const bool done = a.direct && j.p[1].info && ns == 1;
     float m = -INFINITY, l = 0.0f;
-    for (int i = lane; i < ns; i += 64)
-    {
-        const f32x2 e = ml[i];
-        if (e.y != 0.0f) m = fmaxf(m, e.x);
-    }
+    const auto ml = [&](int i) {
+        return i < n0 ? ((gcptr<f32x2>)j.p[0].ml)[pre.at + i * pre.step] : ((gcptr<f32x2>)j.p[1].ml)[own.at + (i - n0) * own.step];
+    };
+    if (!done)
+        for (int i = lane; i < ns; i += 64)
+        {
+            const f32x2 e = ml(i);
+            if (e.y != 0.0f) m = fmaxf(m, e.x);
+        }
     m = max_wave(m);
-    for (int i = lane; i < ns; i += 64)
-    {
-        const f32x2 e = ml[i];
-        const float w = fmaxf(__builtin_amdgcn_exp2f(e.x - (m == -INFINITY ? 0.0f : m)), 0x1p-126f);   // as f above
-        if (sub == 0) wt[local][i] = e.y != 0.0f ? w : -1.0f;      // -1: nothing was written
-        if (e.y != 0.0f) l = fmaf(w, e.y, l);
-    }
+    if (!done)
+        for (int i = lane; i < ns; i += 64)
+        {
+            const f32x2 e = ml(i);
+            const float w = fmaxf(__builtin_amdgcn_exp2f(e.x - (m == -INFINITY ? 0.0f : m)), 0x1p-126f);   // as f above
+            if (sub == 0) wt[local][i] = e.y != 0.0f ? w : -1.0f;      // -1: nothing was written
+            if (e.y != 0.0f) l = fmaf(w, e.y, l);
+        }
     l = group_sum<64>(l);
     __syncthreads();
     f32x4 o{};
-    const gcptr<f32x4> po = (gcptr<f32x4>)(a.po + gr * ns * HD) + lane % LPR;
-    #pragma unroll 4
-    for (int i = sub * SPW + lane / LPR; i < ns; i += WAVES * SPW)
+    if (!done)
     {
-        const float w = wt[local][i];
-        if (w < 0.0f) continue;
-        const f32x4 p = po[(int64_t)i * LPR];
-        #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(w, p[e], o[e]);
+        const gcptr<f32x4> p0 = (gcptr<f32x4>)(j.p[0].po + pre.at * HD) + lane % LPR, p1 = (gcptr<f32x4>)(j.p[1].po + own.at * HD) + lane % LPR;
+        #pragma unroll 4
+        for (int i = sub * SPW + lane / LPR; i < ns; i += WAVES * SPW)
+        {
+            const float w = wt[local][i];
+            if (w < 0.0f) continue;
+            const f32x4 p = i < n0 ? p0[i * pre.step * LPR] : p1[(i - n0) * own.step * LPR];
+            #pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(w, p[e], o[e]);
+        }
     }
     part[wave][lane] = o;
     __syncthreads();
-    if (sub != 0 || lane >= LPR || (int64_t)blockIdx.x * (4 / WAVES) + local >= a.rows_all) return;
+    if (done || sub != 0 || lane >= LPR || (int64_t)blockIdx.x * (4 / WAVES) + local >= a.rows_all) return;
     #pragma unroll
     for (int w = 0; w < WAVES; ++w)
         #pragma unroll
@@ -968,8 +1131,6 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a)
             #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] += p[e];
         }
-    const int64_t tok = gr / a.hq;
-    const int h = (int)(gr - tok * a.hq);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (a.lse && lane == 0) a.lse[gr] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     store_out4<IO>(a, tok, h, 4 * lane, o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -983,37 +1144,65 @@ namespace {
 
 struct Phase
 {
-    int cols;       // 0: k_attn_rows; 1, 2: k_attn_keys with that many column tiles
-    int64_t sets, rows, row_tiles, nsplit;
+    int cols;               // 0: k_attn_rows; 1, 2: k_attn_keys with that many column tiles
+    int64_t sets, rows;     // row sets of `rows` query rows per KV head
+    int64_t row_tiles;      // of a row set
+    int64_t n;              // k_attn_rows: splits; k_attn_keys: slots per KV head
+    bool cut;               // a row's keys may lie in several workgroups
+    int64_t partials;       // partial rows in the workspace
+    int64_t grid;
 };
 
 // How a phase is cut: `sets` row sets of `rows` query rows per KV head against at most `span` keys.
-Phase plan_phase(int64_t sets, int64_t rows, int hk, int hd, int64_t span)
+Phase plan_phase(int64_t sets, int64_t rows, int hk, int hd, int64_t span, bool whole)
 {
-    Phase p;
+    Phase p{};
     // (two column tiles of 256 dimensions do not fit the registers: two row tiles then, whose keys meet in the L2)
     p.cols = rows > 32 ? 0 : rows <= 16 || hd == 256 ? 1 : 2;
     p.sets = sets;
     p.rows = rows;
-    const int64_t per_tile = p.cols ? 16 * p.cols : hd == 256 ? 128 : 256;
-    p.row_tiles = (rows + per_tile - 1) / per_tile;
-    const int64_t base = sets * hk * p.row_tiles;
-    const int64_t want = p.cols ? 4096 : 512, least = p.cols ? 128 : 256;
-    int64_t n = (want + base - 1) / base;
-    const int64_t most = (span + least - 1) / least;
-    if (n > most) n = most;
-    if (n > kMaxSplits / 2) n = kMaxSplits / 2;
-    p.nsplit = n < 1 ? 1 : n;
+    if (p.cols == 0)
+    {
+        const int64_t tile = hd == 256 ? 128 : 256;
+        p.row_tiles = (rows + tile - 1) / tile;
+        const int64_t base = sets * hk * p.row_tiles, most = (span + 255) / 256;
+        // A workgroup fills a CU.  The prefix's are equally long: no more than one round of them (16 x 37 tokens of 16
+        // heads on a prefix of 2048: 6 splits 45 us, 7 splits, 280 workgroups, 55).  Others differ: at least one round.
+        const int64_t fill = whole ? 256 / base : (256 + base - 1) / base;
+        p.n = std::max<int64_t>(1, std::min<int64_t>({ fill, most, kMaxSplits }));
+        p.cut = p.n > 1;
+        p.partials = p.n * sets * rows * hk;
+        p.grid = base * p.n;
+    }
+    else
+    {
+        const int64_t tile = 16 * p.cols;
+        p.row_tiles = (rows + tile - 1) / tile;
+        const int64_t segs = sets * p.row_tiles, units = (span + 127) / 128;
+        // Two workgroups to a CU, as many as are resident; with more segments than that one each, as a slot starts its
+        // segments one after the other.  (64 sequences of 700 to 8100 keys: 512 workgroups 221 us, 1024 225, 2048 232;
+        // 2 sequences of 98765 and 131000: 100, 107, 123.)
+        const int64_t want = std::max<int64_t>(512, std::min<int64_t>(segs * hk, 4096));
+        p.n = std::max<int64_t>(1, std::min<int64_t>({ want / hk, segs * units, kMaxSplits }));
+        p.cut = p.n > 1 && units > 1;
+        p.partials = (p.n + segs) * hk * std::min(tile, rows);
+        p.grid = p.n * hk;
+    }
     return p;
 }
 
 struct Plan
 {
-    Phase prefix, own;      // prefix.nsplit 0: none
-    int64_t splits;
+    Phase prefix, own;      // prefix.n 0: none
     bool join;
     size_t bytes;
 };
+
+size_t phase_bytes(const Phase& p, int hd)
+{
+    const size_t info = p.cols ? ((size_t)p.sets * p.row_tiles * 8 + 255) & ~(size_t)255 : 0;
+    return info + (((size_t)p.partials * (size_t)(hd + 2) * 4 + 255) & ~(size_t)255);
+}
 
 Plan make_plan(int64_t bsz, int64_t seq, int hq, int hk, int hd, int64_t cap, int64_t window, int64_t sinks, int64_t shared)
 {
@@ -1025,11 +1214,10 @@ Plan make_plan(int64_t bsz, int64_t seq, int hq, int hk, int hd, int64_t cap, in
         const int64_t w = window + seq + sinks + 256;
         if (w < span) span = w;
     }
-    p.own = plan_phase(bsz, seq * group, hk, hd, span);
-    if (shared > 0) p.prefix = plan_phase(1, bsz * seq * group, hk, hd, shared);
-    p.splits = p.own.nsplit + p.prefix.nsplit;
-    p.join = p.splits > 1;
-    if (p.join) p.bytes = ((size_t)p.splits * (size_t)(bsz * seq * hq) * (size_t)(hd + 2) * 4 + 255) & ~(size_t)255;
+    p.own = plan_phase(bsz, seq * group, hk, hd, span, false);
+    if (shared > 0) p.prefix = plan_phase(1, bsz * seq * group, hk, hd, shared, true);
+    p.join = shared > 0 || p.own.cut;
+    if (p.join) p.bytes = phase_bytes(p.own, hd) + (shared > 0 ? phase_bytes(p.prefix, hd) : 0);
     return p;
 }
 
@@ -1065,8 +1253,7 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
     if ((hq > 1 && (q_hs < hd || o_hs < hd)) || (tokens > 1 && (q_ts < hd || o_ts < hd)))
         return set_error(EXL3R_EINVAL, "%s: strides shorter than a head", op);
     const Plan p = make_plan(bsz, seq, hq, hk, hd, cap, window, sinks, shared);
-    if (p.own.sets * hk * p.own.row_tiles * p.own.nsplit > 0xffffff || p.prefix.sets * hk * p.prefix.row_tiles * p.prefix.nsplit > 0xffffff ||
-        (p.join && tokens * hq > 0xffffff))
+    if (p.own.grid > 0xffffff || p.prefix.grid > 0xffffff || (p.join && tokens * hq > 0xffffff))
         return set_error(EXL3R_EINVAL, "%s: more than 2^24 workgroups", op);
     if (p.join && (!ws || ((uintptr_t)ws & 255) || ws_bytes < p.bytes))
         return set_error(EXL3R_EINVAL, "%s: the workspace must be 256-byte aligned and hold %zu bytes (%zu given)", op, p.bytes, ws ? ws_bytes : 0);
@@ -1081,9 +1268,6 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
     a.lens = lens;
     a.err = err;
     a.rows_all = tokens * hq;
-    a.po = (float*)ws;
-    a.splits = (int)p.splits;
-    a.pml = p.join ? (float*)ws + p.splits * a.rows_all * hd : nullptr;
     a.q_ts = q_ts; a.q_hs = q_hs; a.o_ts = o_ts; a.o_hs = o_hs;
     a.max_blocks = max_blocks;
     a.num_pages = num_pages;
@@ -1091,7 +1275,7 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
     a.page_shift = __builtin_ctz((unsigned)page_size);
     a.window = window > 0 ? window : 0;
     a.sinks = sinks;
-    a.direct = !p.join;
+    a.direct = shared == 0;
     a.q_vec = aligned16(q) && (hq == 1 || q_hs % 8 == 0) && (tokens == 1 || q_ts % 8 == 0);
     a.o_vec = ((uintptr_t)out & 7) == 0 && (hq == 1 || o_hs % 4 == 0) && (tokens == 1 || o_ts % 4 == 0);
     a.c = scale * 1.4426950408889634f;
@@ -1100,16 +1284,42 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
     auto run = [&](auto T, auto HDC) {
         using IO = decltype(T);
         constexpr int HD = decltype(HDC)::value;
-        auto phase = [&](const Phase& ph, bool whole, int64_t lo, int64_t hi, int64_t split0) {
+        char* place = (char*)ws;
+        auto phase = [&](const Phase& ph, bool whole, int64_t lo, int64_t hi) {
             AttnArgs x = a;
             x.whole = whole;
             x.dom_lo = (int)lo;
             x.dom_hi = (int)hi;
             x.rows = (int)ph.rows;
             x.row_tiles = (int)ph.row_tiles;
-            x.nsplit = (int)ph.nsplit;
-            x.split0 = (int)split0;
-            const int64_t grid = ph.sets * hk * ph.row_tiles * ph.nsplit;
+            Parts& pt = x.parts;
+            const int64_t segs = ph.sets * ph.row_tiles;
+            if (ph.cols)
+            {
+                pt.slots = (int)ph.n;
+                pt.segs = (int)segs;
+                pt.row_tiles = (int)ph.row_tiles;
+                pt.seg_rows = (int)std::min<int64_t>(16 * ph.cols, ph.rows);
+                pt.whole = whole;
+            }
+            else
+            {
+                pt.n = (int)ph.n;
+                x.direct = !p.join;
+            }
+            if (p.join)
+            {
+                char* at = place;
+                if (ph.cols)
+                {
+                    pt.info = (int32_t*)at;
+                    at += (segs * 8 + 255) & ~(int64_t)255;
+                }
+                pt.po = (float*)at;
+                pt.ml = pt.po + ph.partials * hd;
+                place += phase_bytes(ph, hd);
+            }
+            const int64_t grid = ph.grid;
             if (ph.cols == 0)
             {
                 constexpr int W = HD == 256 ? 4 : 8, KT = HD == 256 ? 32 : 64;
@@ -1126,13 +1336,16 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
                 if (page_size < 32) launch(k_attn_keys<IO, HD, 2, true>, (unsigned)grid, 256, 0, st, x);
                 else launch(k_attn_keys<IO, HD, 2, false>, (unsigned)grid, 256, 0, st, x);
             }
+            return pt;
         };
-        if (shared > 0) phase(p.prefix, true, 0, shared, 0);
-        phase(p.own, false, shared, cap, p.prefix.nsplit);
+        JoinArgs j{};
+        if (shared > 0) j.p[0] = phase(p.prefix, true, 0, shared);
+        j.p[1] = phase(p.own, false, shared, cap);
         if (p.join)
         {
-            if (p.splits > 16) launch(k_attn_join<IO, HD, 4>, (unsigned)a.rows_all, 256, 0, st, a);
-            else launch(k_attn_join<IO, HD, 1>, (unsigned)((a.rows_all + 3) / 4), 256, 0, st, a);
+            // Many partial results of few rows: 4 waves each.  (16 + up to 8 of 4096 rows: 12 us so, 9 with one wave.)
+            if (p.own.n + p.prefix.n > 16 && a.rows_all <= 1024) launch(k_attn_join<IO, HD, 4>, (unsigned)a.rows_all, 256, 0, st, a, j);
+            else launch(k_attn_join<IO, HD, 1>, (unsigned)((a.rows_all + 3) / 4), 256, 0, st, a, j);
         }
     };
     auto by_dim = [&](auto T) {
