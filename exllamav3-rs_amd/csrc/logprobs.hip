@@ -16,6 +16,7 @@ constexpr int kLpLanes = 256;
 constexpr int kLpChunks = 4;                                 // chunks of 8 columns per lane and step
 constexpr int kLpStep = kLpLanes * 8 * kLpChunks;            // columns per step of a workgroup
 constexpr int kLpMaxTop = 32;
+constexpr int kLpKeep = 24;                                  // group maxima per lane that stay in registers (196608 columns)
 constexpr int kLpList = 64;                                  // groups read again at most in the usual way
 // Columns ranked at most: in the careful way, those of fewer than kLpMaxTop groups and, of the columns that share the
 // floor's value, fewer than kLpMaxTop and one round of the search.
@@ -43,13 +44,18 @@ __device__ __forceinline__ float lp_max_nan(float a, float b) { return __builtin
 // Order-preserving 32-bit image of a float; -0 maps with +0 and every NaN to the top.
 __device__ __forceinline__ uint32_t lp_order(float v)
 {
-    if (v != v) return 0xffffffffu;
     const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.0f);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return v != v ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 // Larger value, then lower index; below ~0 for every value and index, above 0.
 __device__ __forceinline__ uint64_t lp_key(float v, uint32_t i) { return ((uint64_t)lp_order(v) << 32) | (0xfffffffeu - i); }
 __device__ __forceinline__ uint32_t lp_index(uint64_t k) { return 0xfffffffeu - (uint32_t)k; }
+__device__ __forceinline__ float lp_value(uint64_t k)
+{
+    const uint32_t u = (uint32_t)(k >> 32);
+    if (u == 0xffffffffu) return NAN;
+    return __builtin_bit_cast(float, (u & 0x80000000u) ? u ^ 0x80000000u : ~u);
+}
 
 struct LpSum
 {
@@ -170,13 +176,44 @@ struct LpShared
     uint32_t list[kLpList];
     uint64_t cand[kLpCands];
     int nlist, nabove, ncand, nfound, count[2];
-    uint32_t floor;
 };
 
-// Everything a row's sums and group maxima give: m, l, t in every lane; `groups` maxima at gmax.
+// The order images of a lane's kLpKeep group maxima from group r0 on (0 past the last, below every maximum's): one wait
+// for all of them.
+template <class P>
+__device__ __forceinline__ void lp_maxima(P gmax, int64_t groups, int64_t r0, uint32_t (&k)[kLpKeep])
+{
+    const int tid = threadIdx.x, left = (int)min(groups - r0, (int64_t)kLpKeep * kLpLanes);
+    float v[kLpKeep];
+    #pragma unroll
+    for (int i = 0; i < kLpKeep; ++i) v[i] = gmax[r0 + min(i * kLpLanes, left - kLpLanes) + tid];     // (left: whole steps)
+    #pragma unroll
+    for (int i = 0; i < kLpKeep; ++i) k[i] = i * kLpLanes < left ? lp_order(v[i]) : 0;
+}
+
+// The row's token and its logit, in one lane of the last wave.
+struct LpToken
+{
+    int64_t id = 0;
+    float x = 0.0f;
+};
+template <class IT>
+__device__ __forceinline__ LpToken lp_token(const LpArgs& a, int64_t row)
+{
+    LpToken t;
+    if ((int)threadIdx.x == kLpLanes - 64 && a.tokens)
+    {
+        t.id = a.tokens[row];
+        if (t.id >= 0 && t.id < a.n) t.x = load1(a.x + row * a.ld, IT::code, t.id);
+    }
+    return t;
+}
+
+// Everything a row's sums and group maxima give: m, l, t in every lane; `groups` maxima at gmax, the lane's first ones
+// in kept.
 template <class IT, class P>
 __device__ __forceinline__ void lp_finish(const LpArgs& a, int64_t row, float m, float l, float t, P gmax, int64_t groups,
-                                          LpShared& sh)
+                                          uint32_t (&kept)[kLpKeep], const LpToken& token, LpShared& sh)
 {
     const int tid = threadIdx.x;
     const char* base = a.x + row * a.ld;
@@ -187,76 +224,78 @@ __device__ __forceinline__ void lp_finish(const LpArgs& a, int64_t row, float m,
     {
         if (a.tokens)
         {
-            const int64_t k = a.tokens[row];
+            const int64_t k = token.id;
             if (a.err && (k < 0 || k >= a.vocab)) *a.err = 1;
-            a.logprobs[row] = k < 0 || k >= a.n ? (ll != ll ? NAN : -INFINITY) : log_p(load1(base, IT::code, k));
+            a.logprobs[row] = k < 0 || k >= a.n ? (ll != ll ? NAN : -INFINITY) : log_p(token.x);
         }
         if (a.entropy) a.entropy[row] = (float)(ll - (double)t / l);
     }
     const int top = a.top;
     if (!top) return;
-    // Eight of the lane's maxima at a time: one wait for their loads.
-    constexpr int B = 8;
+    constexpr int64_t ROUND = (int64_t)kLpKeep * kLpLanes;
     uint32_t best = 0;
-    for (int64_t g0 = tid; g0 < groups; g0 += B * kLpLanes)
+    for (int64_t r0 = 0; r0 < groups; r0 += ROUND)
     {
-        float v[B];
+        if (r0 != 0) lp_maxima(gmax, groups, r0, kept);
         #pragma unroll
-        for (int i = 0; i < B; ++i) v[i] = g0 + i * kLpLanes < groups ? gmax[g0 + i * kLpLanes] : -INFINITY;
-        #pragma unroll
-        for (int i = 0; i < B; ++i)
-        {
-            const uint32_t k = lp_order(v[i]);
-            best = k > best ? k : best;
-        }
+        for (int i = 0; i < kLpKeep; ++i) best = max(best, kept[i]);
     }
     ((uint32_t*)sh.best)[tid] = best;
     if (tid == 0) sh.nlist = sh.nabove = sh.ncand = sh.nfound = 0;
     __syncthreads();
-    // The lane whose best has exactly top - 1 others before it (ties by lane) holds the floor.
-    int before = 0;
-    #pragma unroll 8
-    for (int i = 0; i < kLpLanes / 4; ++i)
+    // The floor: the top-th largest of the lanes' best, as far as its upper 20 bits say (sign, exponent, 11 bits of the
+    // fraction): lower by less than 2^-11, a column or two more to rank.  Every wave finds it for itself, bit by bit,
+    // four lanes' best in each lane (ranking all against all took 7 of the kernel's 14 us).
+    uint32_t floor = 0;
     {
-        const u32x4 o = sh.best[i];
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) before += o[j] > best || (o[j] == best && 4 * i + j < tid);
-    }
-    if (before == top - 1) sh.floor = best;
-    __syncthreads();
-    uint32_t floor = sh.floor;
-    // (a lane without a group that reaches the floor has none to list)
-    for (int64_t g0 = tid; g0 < groups && best >= floor; g0 += B * kLpLanes)
-    {
-        float v[B];
-        #pragma unroll
-        for (int i = 0; i < B; ++i) v[i] = g0 + i * kLpLanes < groups ? gmax[g0 + i * kLpLanes] : -INFINITY;
-        #pragma unroll
-        for (int i = 0; i < B; ++i)
+        const u32x4 o = sh.best[tid & 63];
+        for (int b = 31; b >= 12; --b)
         {
-            const int64_t g = g0 + i * kLpLanes;
-            const uint32_t k = lp_order(v[i]);
-            if (g < groups && k >= floor)
-            {
-                const int at = atomicAdd(&sh.nlist, 1);
-                if (at < kLpList) sh.list[at] = (uint32_t)g;
-                if (k > floor) atomicAdd(&sh.nabove, 1);
-            }
+            const uint32_t w = floor | 1u << b;
+            int n = 0;
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) n += __popcll(__ballot(o[j] >= w));
+            floor = n >= top ? w : floor;
         }
+    }
+    // (a lane without a group that reaches the floor has none to list)
+    for (int64_t r0 = 0; r0 < groups && best >= floor; r0 += ROUND)
+    {
+        if (groups > ROUND) lp_maxima(gmax, groups, r0, kept);
+        uint32_t reach = 0, more = 0;
+        #pragma unroll
+        for (int i = 0; i < kLpKeep; ++i)
+        {
+            reach |= kept[i] >= floor ? 1u << i : 0u;
+            more += kept[i] > floor;
+        }
+        if (more) atomicAdd(&sh.nabove, more);
+        for (int at = reach ? atomicAdd(&sh.nlist, __popc(reach)) : 0; reach; reach &= reach - 1, ++at)
+            if (at < kLpList) sh.list[at] = (uint32_t)(r0 + (__ffs(reach) - 1) * kLpLanes + tid);
     }
     __syncthreads();
     const int listed = sh.nlist, above = sh.nabove;
     if (listed <= kLpList)
     {
-        for (int i = tid; i < listed * kLpChunks * 8; i += kLpLanes)
+        constexpr int B = 4;        // (one wait for four of the lane's columns)
+        for (int i0 = tid; i0 < listed * kLpChunks * 8; i0 += B * kLpLanes)
         {
-            const int64_t c = lp_column(sh.list[i / (kLpChunks * 8)], (i / 8) % kLpChunks) + i % 8;
-            const float x = c < a.n ? load1(base, IT::code, c) : 0.0f;
-            if (c < a.n && lp_order(x) >= floor)
+            float x[B];
+            int64_t c[B];
+            #pragma unroll
+            for (int u = 0; u < B; ++u)
             {
-                const int at = atomicAdd(&sh.ncand, 1);
-                if (at < kLpCands) sh.cand[at] = lp_key(x, (uint32_t)c);
+                const int i = i0 + u * kLpLanes;
+                c[u] = i < listed * kLpChunks * 8 ? lp_column(sh.list[i / (kLpChunks * 8)], (i / 8) % kLpChunks) + i % 8 : a.n;
+                x[u] = c[u] < a.n ? load1(base, IT::code, c[u]) : 0.0f;
             }
+            #pragma unroll
+            for (int u = 0; u < B; ++u)
+                if (c[u] < a.n && lp_order(x[u]) >= floor)
+                {
+                    const int at = atomicAdd(&sh.ncand, 1);
+                    if (at < kLpCands) sh.cand[at] = lp_key(x[u], (uint32_t)c[u]);
+                }
         }
     }
     __syncthreads();
@@ -314,12 +353,12 @@ __device__ __forceinline__ void lp_finish(const LpArgs& a, int64_t row, float m,
     {
         const uint64_t k = sh.cand[i];
         int rank = 0;
+        #pragma unroll 8
         for (int j = 0; j < n; ++j) rank += sh.cand[j] > k;
         if (rank < top)
         {
-            const int64_t c = lp_index(k);
-            a.top_ids[row * top + rank] = c;
-            a.top_logprobs[row * top + rank] = log_p(load1(base, IT::code, c));
+            a.top_ids[row * top + rank] = lp_index(k);
+            a.top_logprobs[row * top + rank] = log_p(lp_value(k));
         }
     }
 }
@@ -351,8 +390,12 @@ template <class IT>
 __global__ __launch_bounds__(kLpLanes) void k_lp_join(LpArgs a)
 {
     __shared__ LpShared sh;
-    const int64_t row = blockIdx.x;
     __shared__ float w[kLpLanes / 64][3];
+    const int64_t row = blockIdx.x;
+    const gcptr<float> gmax = (gcptr<float>)a.gmax + row * a.groups;
+    const LpToken token = lp_token<IT>(a, row);
+    uint32_t kept[kLpKeep] = {};
+    if (a.top) lp_maxima(gmax, a.groups, 0, kept);
     LpSum s;
     if ((int)threadIdx.x < a.slices)
     {
@@ -360,7 +403,7 @@ __global__ __launch_bounds__(kLpLanes) void k_lp_join(LpArgs a)
         s.m = p[0]; s.l = p[1]; s.t = p[2];
     }
     s = lp_block_sum(s, w);
-    lp_finish<IT>(a, row, s.m, s.l, s.t, (gcptr<float>)a.gmax + row * a.groups, a.groups, sh);
+    lp_finish<IT>(a, row, s.m, s.l, s.t, gmax, a.groups, kept, token, sh);
 }
 
 // Many rows: a workgroup per row, its group maxima in LDS.
@@ -373,6 +416,7 @@ __global__ __launch_bounds__(kLpLanes) void k_lp_rows(LpArgs a)
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const char* base = a.x + row * a.ld;
+    const LpToken token = lp_token<IT>(a, row);
     LpSum s;
     for (int64_t i = 0; i * kLpStep < a.n; ++i)
     {
@@ -380,7 +424,9 @@ __global__ __launch_bounds__(kLpLanes) void k_lp_rows(LpArgs a)
         if (a.top) gmax[i * kLpLanes + tid] = gm;
     }
     s = lp_block_sum(s, w);
-    lp_finish<IT>(a, row, s.m, s.l, s.t, gmax, a.groups, sh);
+    uint32_t kept[kLpKeep] = {};
+    if (a.top) lp_maxima(gmax, a.groups, 0, kept);
+    lp_finish<IT>(a, row, s.m, s.l, s.t, gmax, a.groups, kept, token, sh);
 }
 
 }  // namespace exl3r
@@ -401,7 +447,7 @@ LpPlan lp_plan(int64_t rows, int64_t n)
     LpPlan p;
     const int64_t all = (n + kLpStep - 1) / kLpStep;
     p.groups = all * kLpLanes;
-    p.by_rows = rows >= 512 && p.groups * 4 <= 64 << 10;
+    p.by_rows = rows >= 256 && p.groups * 4 <= 64 << 10;
     p.steps = (all + 255) / 256;
     p.slices = (all + p.steps - 1) / p.steps;
     p.part_bytes = ((size_t)rows * p.slices * 12 + 255) & ~(size_t)255;
