@@ -631,6 +631,111 @@ void rope_paged_kv(const Tensor& q, const Tensor& out_q, const Tensor& k, const 
                                   (const int32_t*)cache_seqlens.data, err_flag, ptr(cs_table), s.get()));
 }
 
+namespace
+{
+
+// The arguments of both forms; shared_len < 0: paged_attn.
+void attention(const char* op, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+               const Tensor& cache_seqlens, const Tensor& out, int64_t shared_len, float scale, int window, int sinks,
+               const Tensor* lse, int32_t* err_flag, const DeviceBuffer* workspace, const Stream& s)
+{
+    const auto need = [&](bool ok, const char* what) {
+        if (!ok) throw Error(EXL3R_EINVAL, std::string(op) + ": " + what);
+    };
+    need(q.dim() == 4 && out.shape == q.shape, "q and out must be (bsz, seq_len, heads, head_dim)");
+    const int64_t bsz = q.size(0), seq = q.size(1), hq = q.size(2), hd = q.size(3);
+    for (const Tensor* t : { &q, &out })
+        need(t->stride(3) == 1 && (bsz <= 1 || seq <= 1 || t->stride(0) == seq * t->stride(1)),
+             "q / out: dense innermost dim and batch stride seq_len * token stride");
+    need(k_cache.dim() == 4 && k_cache.shape == v_cache.shape && k_cache.size(3) == hd && k_cache.is_contiguous() &&
+             v_cache.is_contiguous(),
+         "caches must be contiguous (pages, page_size, kv_heads, head_dim)");
+    need(k_cache.dtype == q.dtype && v_cache.dtype == q.dtype && out.dtype == q.dtype, "q, out and the caches must share a dtype");
+    need(block_table.dim() == 2 && block_table.dtype == DType::I32 && block_table.size(0) == bsz && block_table.is_contiguous() &&
+             cache_seqlens.dtype == DType::I32 && cache_seqlens.numel() == bsz && cache_seqlens.is_contiguous(),
+         "block_table (bsz, max_blocks) and cache_seqlens (bsz) must be contiguous int32");
+    need(!lse || (lse->dtype == DType::F32 && lse->numel() == bsz * seq * hq && lse->is_contiguous()),
+         "lse must be a contiguous float32 (bsz, seq_len, heads)");
+    const float sc = scale > 0.0f ? scale : (float)(1.0 / std::sqrt((double)hd));
+    const int64_t qs = q.stride(seq == 1 ? 0 : 1), os = out.stride(seq == 1 ? 0 : 1);
+    void* const ws = workspace ? workspace->data() : nullptr;
+    const size_t wb = workspace ? workspace->bytes() : 0;
+    const auto *bt = (const int32_t*)block_table.data, *cl = (const int32_t*)cache_seqlens.data;
+    float* const l = lse ? (float*)lse->data : nullptr;
+    if (shared_len < 0)
+        check_abi(exl3r_paged_attn(q.data, qs, q.stride(2), (int)hq, k_cache.data, v_cache.data, (int)k_cache.size(2),
+                                   (int)k_cache.size(1), k_cache.size(0), bt, block_table.size(1), cl, code(q.dtype), bsz, seq,
+                                   (int)hd, sc, window, sinks, out.data, os, out.stride(2), l, err_flag, ws, wb, s.get()));
+    else
+        check_abi(exl3r_paged_attn_shared(q.data, qs, q.stride(2), (int)hq, k_cache.data, v_cache.data, (int)k_cache.size(2),
+                                          (int)k_cache.size(1), k_cache.size(0), bt, block_table.size(1), cl, shared_len,
+                                          code(q.dtype), bsz, seq, (int)hd, sc, window, sinks, out.data, os, out.stride(2), l,
+                                          err_flag, ws, wb, s.get()));
+}
+
+}  // namespace
+
+void paged_attn(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                const Tensor& cache_seqlens, const Tensor& out, float scale, int window, int sinks, const Tensor* lse,
+                int32_t* err_flag, const DeviceBuffer* workspace, const Stream& s)
+{
+    attention("paged_attn", q, k_cache, v_cache, block_table, cache_seqlens, out, -1, scale, window, sinks, lse, err_flag,
+              workspace, s);
+}
+
+void paged_attn_shared(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                       const Tensor& cache_seqlens, const Tensor& out, int64_t shared_len, float scale, int window,
+                       int sinks, const Tensor* lse, int32_t* err_flag, const DeviceBuffer* workspace, const Stream& s)
+{
+    require(shared_len >= 0, "paged_attn_shared: shared_len must be 0 or more");
+    attention("paged_attn_shared", q, k_cache, v_cache, block_table, cache_seqlens, out, shared_len, scale, window, sinks, lse,
+              err_flag, workspace, s);
+}
+
+size_t paged_attn_workspace_bytes(const Tensor& q, const Tensor& k_cache, const Tensor& block_table, int64_t shared_len)
+{
+    require(q.dim() == 4 && k_cache.dim() == 4 && block_table.dim() == 2,
+            "paged_attn_workspace_bytes: q and k_cache have 4 dimensions, block_table 2");
+    return exl3r_paged_attn_workspace_bytes(q.size(0), q.size(1), (int)q.size(2), (int)k_cache.size(2), (int)q.size(3),
+                                            (int)k_cache.size(1), block_table.size(1), shared_len);
+}
+
+void token_logprobs(const Tensor& logits, const Tensor* tokens, const Tensor* logprobs, const Tensor* entropy,
+                    const Tensor* top_ids, const Tensor* top_logprobs, int max_logit, int32_t* err_flag,
+                    const DeviceBuffer* workspace, const Stream& s)
+{
+    int64_t rows, vocab, ld;
+    logits.rows_view(rows, vocab, ld);
+    require(!tokens == !logprobs, "token_logprobs: tokens and logprobs go together");
+    require(!top_ids == !top_logprobs, "token_logprobs: top_ids and top_logprobs go together");
+    require(!tokens || (tokens->dtype == DType::I64 && tokens->numel() == rows && tokens->is_contiguous()),
+            "token_logprobs: tokens must be contiguous int64 with one entry per row");
+    for (const Tensor* t : { logprobs, entropy })
+        require(!t || (t->dtype == DType::F32 && t->numel() == rows && t->is_contiguous()),
+                "token_logprobs: logprobs and entropy must be contiguous float32 with one entry per row");
+    int64_t k = 0;
+    if (top_ids)
+    {
+        require(top_ids->dtype == DType::I64 && top_logprobs->dtype == DType::F32 && top_ids->dim() > 0 &&
+                    top_ids->shape == top_logprobs->shape && top_ids->is_contiguous() && top_logprobs->is_contiguous(),
+                "token_logprobs: top_ids (int64) and top_logprobs (float32) must be contiguous and alike");
+        k = top_ids->size(-1);
+        require(top_ids->numel() == rows * k && k <= 0x7fffffff, "token_logprobs: top_ids must have one row per logits row");
+    }
+    check_abi(exl3r_token_logprobs(logits.data, code(logits.dtype), rows, vocab, ld, max_logit, (const int64_t*)ptr(tokens),
+                                   logprobs ? (float*)logprobs->data : nullptr, entropy ? (float*)entropy->data : nullptr,
+                                   (int)k, top_ids ? (int64_t*)top_ids->data : nullptr,
+                                   top_logprobs ? (float*)top_logprobs->data : nullptr, err_flag,
+                                   workspace ? workspace->data() : nullptr, workspace ? workspace->bytes() : 0, s.get()));
+}
+
+size_t token_logprobs_workspace_bytes(const Tensor& logits)
+{
+    int64_t rows, vocab, ld;
+    logits.rows_view(rows, vocab, ld);
+    return exl3r_token_logprobs_workspace_bytes(rows, vocab);
+}
+
 void rope_paged_kv_had(const Tensor& q, const Tensor& out_q, const Tensor& k, const Tensor* out_k, const Tensor& v,
                        const Tensor& inv_freq, int64_t position, const Tensor* positions, const Tensor* q_norm,
                        const Tensor* k_norm, float norm_eps, float norm_constant_bias, RopeStyle rope_mode,

@@ -8,7 +8,9 @@
 //   exl3r::ffi::rms_norm / rms_norm_res_in / silu_mul / gelu_mul / rope  <- src/ffi.rs:293-333, 464-503
 //   exl3r::ffi::gated_rms_norm / mul_sigmoid_ / deinterleave_qg          <- src/ffi.rs:479-483, 616-624
 //   exl3r::ffi::rope_paged_kv                                            <- rope + paged append, src/modules.rs:666-704
+//   exl3r::ffi::paged_attn / paged_attn_shared                           (attention over that cache)
 //   exl3r::ffi::argmax_sample / gumbel_sample / gumbel_noise             <- src/ffi.rs:521-535, src/generator.rs:1596
+//   exl3r::ffi::token_logprobs                                           (log probabilities of the same logits)
 //   exl3r::ffi::had_r_128 / rms_norm_had / act_mul_had / rope_had        <- src/ffi.rs:606-607, src/modules.rs:224-231
 //   exl3r::ffi::rope_cs_table / rope_cs                                  <- rope() with the sin / cos hoisted per forward
 //   exl3r::ffi::rope_qg                                                  <- deinterleave_qg + rope, src/modules.rs:637-681
@@ -222,6 +224,20 @@ void rope_paged_kv(const Tensor& q, const Tensor& out_q, const Tensor& k, const 
                    const Tensor* k_norm, float norm_eps, float norm_constant_bias, RopeStyle rope_mode, float attn_factor,
                    const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& cache_seqlens,
                    int32_t* err_flag, const Stream& s, const Tensor* cs_table = nullptr);
+// Causal attention of q (bsz, seq_len, heads, head_dim) over the caches that rope_paged_kv() filled, called after it
+// with the same block_table and cache_seqlens: token s of sequence b sees the positions up to cache_seqlens[b] + s; with
+// window > 0 only the last `window` of them and the first `sinks`.  scale <= 0: 1 / sqrt(head_dim).  lse, null or
+// float32 [bsz * seq_len * heads]: the scores' log-sum-exp.  workspace: paged_attn_workspace_bytes() bytes (any
+// contents; not shared by calls that overlap), may be null where that is 0.
+void paged_attn(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                const Tensor& cache_seqlens, const Tensor& out, float scale, int window, int sinks, const Tensor* lse,
+                int32_t* err_flag, const DeviceBuffer* workspace, const Stream& s);
+// paged_attn() of sequences whose first shared_len positions (whole pages) lie on the same pages: those keys are read
+// once for the whole batch, through the block table's first row.
+void paged_attn_shared(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
+                       const Tensor& cache_seqlens, const Tensor& out, int64_t shared_len, float scale, int window,
+                       int sinks, const Tensor* lse, int32_t* err_flag, const DeviceBuffer* workspace, const Stream& s);
+size_t paged_attn_workspace_bytes(const Tensor& q, const Tensor& k_cache, const Tensor& block_table, int64_t shared_len = 0);
 // src/ffi.rs:521-525 (and the generator's batched argmax, src/generator.rs:1596): ids[i] = first index of the
 // maximum of logits[i, :max_logit] (whole row when max_logit <= 0), NaN maximal; ids int64 [rows].
 void argmax_sample(const Tensor& logits, const Tensor& ids, int max_logit, const Stream& s);
@@ -235,6 +251,14 @@ void argmax_sample_ws(const Tensor& logits, const Tensor& ids, int max_logit, co
                       const Stream& s);
 void gumbel_sample_ws(const Tensor& logits, const Tensor& ids, int max_logit, uint32_t random,
                       const DeviceBuffer& workspace, const Stream& s);
+// logprobs[i] = log softmax(logits[i, :max_logit])[tokens[i]] (both may be null), entropy[i] (or null) that
+// distribution's entropy, and its top_ids.size(-1) most probable tokens (both tops may be null), ties to the lowest
+// index, with their log probabilities, in one read of the logits.  float32 outputs, int64 tokens and ids; workspace:
+// token_logprobs_workspace_bytes() bytes as above.
+void token_logprobs(const Tensor& logits, const Tensor* tokens, const Tensor* logprobs, const Tensor* entropy,
+                    const Tensor* top_ids, const Tensor* top_logprobs, int max_logit, int32_t* err_flag,
+                    const DeviceBuffer* workspace, const Stream& s);
+size_t token_logprobs_workspace_bytes(const Tensor& logits);
 // src/ffi.rs:531-535: out = x + the Gumbel noise gumbel_sample adds (out may be x).
 void gumbel_noise(const Tensor& x, const Tensor& out, uint32_t random, const Stream& s);
 // src/ffi.rs:606-607: the EXL3 linear's random-Hadamard rotation of [rows, cols] f16 / f32 x into out
