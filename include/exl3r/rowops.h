@@ -657,7 +657,7 @@ EXL3R_API size_t exl3r_paged_attn_workspace_bytes(int64_t bsz, int64_t seq_len, 
  *   logprobs[r] = x[r, tokens[r]] - z;   entropy[r] = -sum_c P_c ln P_c, P_c = exp(x[r, c] - z);
  *   top_ids[r, i], top_logprobs[r, i]: the top_k largest logits' columns in falling order, equal ones by rising
  *   column (exl3r_argmax_sample's order: NaN largest, -0 equal to +0), and their log probabilities.
- * fp32 with the row's sums joined in fp64.  Columns from max_logit on are masked out as in exl3r_argmax_sample.  A
+ * fp32 sums, their logarithm and the differences in fp64.  Columns from max_logit on are masked out as in exl3r_argmax_sample.  A
  * token outside [0, n) has log probability -inf; one outside [0, vocab) also stores 1 to *err_flag (device int32, or
  * NULL).  A NaN or +inf among a row's logits, or all of them -inf, make its results NaN (top_ids stay defined).
  *   logits: [rows, vocab], row stride ld elements, F16/BF16/F32.  tokens: int64 [rows], or NULL: logprobs is not

@@ -93,3 +93,13 @@ def test_logprobs_nothing_to_do():
     assert logprobs(rows=0, k=40) == exl3r.EINVAL
     f = exl3r.load().exl3r_token_logprobs_workspace_bytes
     assert f(0, 5) == 0 and f(5, 0) == 0 and f(1 << 40, 5) == 0 and f(64, 151936) % 256 == 0 and f(64, 151936) > 0
+
+
+@pytest.mark.parametrize("rows", [1, 64, 300])
+def test_logprobs_workspace_for_fewer_columns(rows):
+    """A workspace for all columns serves every max_logit: also where a wider slice makes fewer slices."""
+    sizes = [exl3r.load().exl3r_token_logprobs_workspace_bytes(rows, steps * 8192) for steps in (1, 19, 64, 65, 255, 256, 257, 512, 513)]
+    if rows < 256:
+        assert sizes == sorted(sizes)
+    else:
+        assert sizes[:3] == [0, 0, 0] and sizes == sorted(sizes)
