@@ -494,7 +494,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 256 ? 1 : 2) void k_attn_rows(Att
     #pragma unroll
     for (int t = 0; t < HD / 32; ++t) o[t] = f32x16{};
     float m = -INFINITY, l = 0.0f;
-    const float slack = kSlack / a.c;
+    const float slack = fminf(kSlack / a.c, 1e38f);
     f32x16 s[NS];
     u32x4 pf[2 * NS];       // P of 16 keys each
     const auto softmax = [&](int i, uint64_t ok, bool part) {
@@ -829,7 +829,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_attn_keys(AttnArgs a
     }
     const int64_t share = uniform64((total + a.parts.slots - 1) / a.parts.slots), x0 = slot * share, x1 = min(x0 + share, total);
     if (x0 >= total) return;
-    const float slack = kSlack / a.c;
+    const float slack = fminf(kSlack / a.c, 1e38f);
     for (;; ++g)
     {
     if (segs != 1) enter(g);
@@ -1246,9 +1246,12 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
         return set_error(EXL3R_EINVAL, "%s: page_size %d is not a power of two", op, page_size);
     if (num_pages <= 0 || num_pages > 0x7fffffffLL || max_blocks <= 0)
         return set_error(EXL3R_EINVAL, "%s: invalid cache num_pages=%lld max_blocks_per_seq=%lld", op, (long long)num_pages, (long long)max_blocks);
-    if (!(scale > 0.0f) || scale > 3.0e38f) return set_error(EXL3R_EINVAL, "%s: scale must be positive and finite", op);
+    if (!(scale > 0.0f) || scale > 2.0e38f)     // (scale log2 e is finite too)
+        return set_error(EXL3R_EINVAL, "%s: scale must be positive and finite", op);
     if (sinks < 0 || (window <= 0 && sinks != 0))
         return set_error(EXL3R_EINVAL, "%s: sinks (%d) must be 0 or more, and 0 without a window", op, sinks);
+    if (hk > (1 << 22) / hd)        // (64 of a cache's rows are indexed in 32 bits)
+        return set_error(EXL3R_EINVAL, "%s: KV heads of more than 2^22 elements together", op);
     if (bsz == 0 || seq == 0) return EXL3R_OK;
     const int64_t group = hq / hk;
     if (max_blocks > 0x7fffffc0LL / page_size || bsz > 0x7fffffffLL || seq > 0x7fffffffLL || bsz * seq > 0x7fffffffLL / hq)
@@ -1264,7 +1267,8 @@ int attn_entry(const char* op, const void* q, int64_t q_ts, int64_t q_hs, int hq
     if ((hq > 1 && (q_hs < hd || o_hs < hd)) || (tokens > 1 && (q_ts < hd || o_ts < hd)))
         return set_error(EXL3R_EINVAL, "%s: strides shorter than a head", op);
     const Plan p = make_plan(bsz, seq, hq, hk, hd, cap, window, sinks, shared);
-    if (p.own.grid > 0xffffff || p.prefix.grid > 0xffffff || (p.join && tokens * hq > 0xffffff))
+    // (2^23: a launch has fewer than 2^32 threads, 512 in a workgroup)
+    if (p.own.grid > 0x7fffff || p.prefix.grid > 0x7fffff || (p.join && tokens * hq > 0xffffff))
         return set_error(EXL3R_EINVAL, "%s: more than 2^24 workgroups", op);
     if (p.join && (!ws || ((uintptr_t)ws & 255) || ws_bytes < p.bytes))
         return set_error(EXL3R_EINVAL, "%s: the workspace must be 256-byte aligned and hold %zu bytes (%zu given)", op, p.bytes, ws ? ws_bytes : 0);

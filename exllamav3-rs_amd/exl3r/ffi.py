@@ -665,6 +665,8 @@ def _paged_attn(shared_len, q, k_cache, v_cache, block_table, cache_seqlens, out
     for t in (k_cache, v_cache, block_table, cache_seqlens, out, lse, err_flag):
         if t is not None and t.device != q.device:
             raise ValueError("every tensor must be on the device of q")
+    if not q.is_cuda:
+        raise ValueError("q must be on the GPU")
     # a batch of one-token sequences may lie at any batch stride
     qs, os = (t.stride(0) if seq == 1 else t.stride(1) for t in (q, out))
     wp, wb = _ws_args(workspace, q)
@@ -738,6 +740,8 @@ def token_logprobs(logits, tokens, logprobs, entropy=None, top_ids=None, top_log
     for t in (tokens, logprobs, entropy, top_ids, top_logprobs, err_flag):
         if t is not None and t.device != logits.device:
             raise ValueError("every tensor must be on the device of the logits")
+    if not logits.is_cuda:
+        raise ValueError("the logits must be on the GPU")
     wp, wb = _ws_args(workspace, logits)
     with _on(logits):
         check(load().exl3r_token_logprobs(_ptr(logits), dtype_code(logits), rows, vocab, ld, int(max_logit), _ptr(tokens),

@@ -614,11 +614,12 @@ EXL3R_API int exl3r_act_mul_had(int act, const void* x, const void* y, int in_dt
  *        strides is allowed).  head_dim 64, 128 or 256; num_heads_q a multiple of num_heads_kv, query head h
  *        reading KV head h / (num_heads_q / num_heads_kv).
  *   k_cache, v_cache, page_size, num_pages, block_table, max_blocks_per_seq: as exl3r_rope_paged_kv (16-byte
- *        aligned).  max_blocks_per_seq * page_size below 2^31.
+ *        aligned).  max_blocks_per_seq * page_size and bsz * seq_len * num_heads_q below 2^31, num_heads_kv * head_dim
+ *        at most 2^22.
  *   err_flag: NULL or a device int32; 1 is stored for a token whose position is negative or past its block table
  *        (it sees the keys that the table holds) and for a visible key whose page is outside [0, num_pages) (it is
  *        taken as not visible).
- *   scale: positive and finite (1 / sqrt(head_dim) as a rule).  sinks must be 0 without a window.
+ *   scale: positive, at most 2e38 (1 / sqrt(head_dim) as a rule).  sinks must be 0 without a window.
  *   workspace: exl3r_paged_attn_workspace_bytes() bytes of device memory, 256-byte aligned (NULL where that is 0),
  *        for the partial results of long key ranges cut over workgroups.  It needs no initial value and keeps none;
  *        calls that share one must not overlap.

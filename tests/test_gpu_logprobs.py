@@ -247,3 +247,11 @@ def test_wrapper_refusals():
                      ((x.long(), tok, lp), dict(workspace=ws))):
         with pytest.raises(Exl3rError):
             ffi.token_logprobs(*args, **kw)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,k", [(260, 524288, "f16", 5), (257, 524289, "bf16", 0), (3, 700001, "f16", 32),
+                                                (255, 4096, "f32", 3), (256, 4096, "f32", 3)])
+def test_where_the_kernel_changes(rows, vocab, dtype, k):
+    """The most group maxima that a row keeps in LDS and one step more, more than a lane keeps in registers, and the rows
+    from which on a workgroup has one."""
+    check(logits(rows, vocab, dtype, 11), tokens_of(rows, vocab, 12), k, tag=f"{rows}x{vocab} {dtype} k{k}")

@@ -88,3 +88,10 @@ def test_a_larger_workspace_from_the_whole_table():
         ffi.paged_attn(q, kc, vc, table, sl, out, window=window, workspace=ws)
         torch.cuda.synchronize()
         compare((out, None), exact(q, kc, vc, table, sl, window=window), f"window {window}")
+
+
+@pytest.mark.parametrize("seq", [1, 40])
+@pytest.mark.parametrize("scale", [1e-40, 1e-30, 1.0, 30.0])
+def test_scales(seq, scale):
+    a = build([300, 7], seq, 4, 2, 64, F16, 32, seed=45, std=0.5)
+    compare(call(*a, scale=scale), exact(*a, scale=scale), f"scale {scale}")

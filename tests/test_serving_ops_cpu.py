@@ -103,3 +103,26 @@ def test_logprobs_workspace_for_fewer_columns(rows):
         assert sizes == sorted(sizes)
     else:
         assert sizes[:3] == [0, 0, 0] and sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("what,change", [("2^22", dict(hk=1 << 16, hq=1 << 16)), ("scale", dict(scale=2.5e38)),
+                                         ("workgroups", dict(bsz=1 << 12, seq=1 << 14, hq=16, hk=16, hd=256, qts=4096, qhs=256, ots=4096, ohs=256))])
+def test_attention_size_limits(what, change):
+    assert attn(**change) == exl3r.EINVAL
+    assert what in err(), err()
+
+
+def test_wrappers_refuse_host_tensors():
+    import torch
+
+    import exl3r.ffi as ffi
+
+    q, kc = torch.zeros(1, 1, 4, 64).half(), torch.zeros(4, 16, 2, 64).half()
+    table, lens = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for stream in (None, 0):
+        with pytest.raises(ValueError, match="GPU"):
+            ffi.paged_attn(q, kc, kc, table, lens, torch.zeros_like(q), stream=stream)
+        with pytest.raises(ValueError, match="GPU"):
+            ffi.paged_attn_shared(q, kc, kc, table, lens, torch.zeros_like(q), 16, stream=stream)
+        with pytest.raises(ValueError, match="GPU"):
+            ffi.token_logprobs(torch.zeros(2, 100), torch.zeros(2, dtype=torch.int64), torch.zeros(2), stream=stream)
