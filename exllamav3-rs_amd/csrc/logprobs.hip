@@ -122,24 +122,32 @@ __device__ __forceinline__ float lp_step(const LpArgs& a, const char* base, int6
             for (int j = 0; j < 8; ++j) x[8 * u + j] = f[j];
         }
     }
-    else
+    else if (a.n >= 8)
     {
+        // The row's last columns: a chunk past the end is read so that it ends there, without what belongs to the chunk
+        // before (the sums and the maximum ask for no order).
+        typename IT::Vec v[kLpChunks];
+        #pragma unroll
+        for (int u = 0; u < kLpChunks; ++u) v[u] = load_chunk<IT, false>(base, min(lp_column(g, u), a.n - 8));
         #pragma unroll
         for (int u = 0; u < kLpChunks; ++u)
         {
-            const int64_t c = lp_column(g, u);
+            const int64_t c = lp_column(g, u), at = min(c, a.n - 8);
             float f[8];
+            unpack8<IT>(v[u], f);
             #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = -INFINITY;
-            if (c + 8 <= a.n) unpack8<IT>(load_chunk<IT, VEC>(base, c), f);
-            else
-            {
-                #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c + j < a.n) f[j] = load1(base, IT::code, c + j);
-            }
+            for (int j = 0; j < 8; ++j) x[8 * u + j] = at + j >= c ? f[j] : -INFINITY;
+        }
+    }
+    else
+    {
+        #pragma unroll
+        for (int j = 0; j < 8 * kLpChunks; ++j) x[j] = -INFINITY;
+        if (g == 0)
+        {
             #pragma unroll
-            for (int j = 0; j < 8; ++j) x[8 * u + j] = f[j];
+            for (int j = 0; j < 8; ++j)
+                if (j < a.n) x[j] = load1(base, IT::code, j);
         }
     }
     float gm = x[0];
