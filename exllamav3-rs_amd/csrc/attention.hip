@@ -452,13 +452,14 @@ __device__ __forceinline__ void flag_positions(const AttnArgs& a, int p)
 // each SIMD) run one slot behind 0 .. 3, so that one wave of a SIMD is at the matrix cores while the other is at the
 // VALU: in step, both wait for the same unit.
 // 256 rows and tiles of 64 keys: 113 KB of LDS and 242 registers, one workgroup per CU.  Every byte of K and V read from
-// LDS then feeds 32 rows and every byte from the L2 256; rows of 128 in two workgroups per CU took 341 us for 295.  Heads
-// of 256 have o and Q of 32 rows in 192 registers: one wave per SIMD, 128 rows, tiles of 32.
-// Measured: 4096 tokens of 64 heads of 128 on 8 KV heads, bf16, 295 us, 930 TFLOP/s of the visible half; 3 x 511 tokens of
-// 16 heads of 256 on 2, on top of 1800 to 5300 keys, 204 us, 535.  Bound by the softmax's slot: of the ~4390 cycles of a
-// tile the products of both waves take 2 x 1320, and a softmax (1230), its loads and LDS writes (820) and two barriers
-// are longer than the other wave's products: the matrix cores are busy for 45% of a CU's time (heads of 256, nothing
-// beside a wave's softmax: 29%, and 75% of the CUs busy: sequences of different lengths).
+// LDS then feeds 32 rows and every byte from the L2 256; rows of 128 in two workgroups per CU took 341 us for 295.
+// Measured: 4096 tokens of 64 heads of 128 on 8 KV heads, bf16, 295 us, 930 TFLOP/s of the visible half.  Bound by the
+// softmax's slot: of the ~4390 cycles of a tile the products of both waves take 2 x 1320, and a softmax (1230), its loads
+// and LDS writes (820) and two barriers are longer than the other wave's products: the matrix cores are busy for 45% of
+// a CU's time.
+// Heads of 256 have o and Q of 32 rows in 192 registers: one wave per SIMD, 128 rows, tiles of 32, and products and softmax
+// of the same wave interleaved, two tiles of loads under way (4 x 4096 tokens of 16 heads on 2, bf16: 712 us, 773 TFLOP/s;
+// with one tile 733, products and softmax in turn 783).  Pages of 16 keys cost it the lookup of every row: 803 us.
 template <class IO, int HD, int WAVES, int KT, bool SMALL>
 __global__ __launch_bounds__(WAVES * 64, HD == 256 ? 1 : 2) void k_attn_rows(AttnArgs a)
 {
@@ -552,7 +553,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 256 ? 1 : 2) void k_attn_rows(Att
         u32x4 ks[STEPS], vs[STEPS];
         const uint32_t row_bytes = (uint32_t)a.hk * (HD * 2);
         const int in_page = (1 << a.page_shift) - 1, last_page = (tl.khi - 1) >> a.page_shift;
-        uint64_t ok0 = 0, ok1 = 0, ok2 = 0;      // the visible keys of the last three tiles loaded that have a page
+        uint64_t ok0 = 0, ok1 = 0, ok2 = 0, ok3 = 0;      // the visible keys of the last tiles loaded that have a page
         bool bad = false;
         int entry = 0, ahead = 0, il = t0;       // (SMALL: a key's page each) page of tile il, of the page after it
         int64_t off = 0;
@@ -567,7 +568,8 @@ __global__ __launch_bounds__(WAVES * 64, HD == 256 ? 1 : 2) void k_attn_rows(Att
         if constexpr (SMALL) entry = page_entry(a, table, tile_key(t0) + (lane & (KT - 1)), tl.khi);
         else enter_page(tile_key(t0), __builtin_amdgcn_readfirstlane(((gcptr<int32_t>)table)[tile_key(t0) >> a.page_shift]));
         const uint32_t lane_off = tid / (HD / 8) * row_bytes + tid % (HD / 8) * 16;
-        const auto load = [&]() {
+        const auto load_into = [&](u32x4 (&ks)[STEPS], u32x4 (&vs)[STEPS]) __attribute__((always_inline)) {
+            ok3 = ok2;
             ok2 = ok1;
             ok1 = ok0;
             if constexpr (SMALL)
@@ -603,17 +605,126 @@ __global__ __launch_bounds__(WAVES * 64, HD == 256 ? 1 : 2) void k_attn_rows(Att
             }
         };
         // The tile loaded last, tile i, into stage st: clean where not every row sees all of it.
-        const auto write = [&](int i, char* st) {
+        const auto load = [&]() { load_into(ks, vs); };
+        const auto clean = [&](int i, u32x4 (&ks)[STEPS], u32x4 (&vs)[STEPS], uint64_t ok) {
             i = min(i, t1 - 1);
-            if (i < gf0 || i >= gf1 || ok0 != FULL)
+            if (i < gf0 || i >= gf1 || ok != FULL)
             {
-                uint64_t seen = ok0;
+                uint64_t seen = ok;
                 if (!SMALL) seen &= __ballot(key_seen(a, tl, tile_key(i) + (lane & (KT - 1)), gmin));
                 if (clean_tile<IO, HD, STEPS, LANES>(ks, vs, seen, tid)) odd = 1;
             }
+        };
+        const auto write = [&](int i, char* st) {
+            clean(i, ks, vs, ok0);
             write_tile<HD, STEPS, LANES, RV>(ks, vs, tid, st, st + KT * RK);
         };
 
+        if constexpr (WAVES == 4)
+        {
+            // One wave per SIMD: its own products and softmax overlap.  A step multiplies the scores of tile i + 1, with the LDS
+            // writes of tile i + 2 between the MFMAs, then o += V(i) P(i) with the softmax of tile i + 1 between them: both
+            // take about as long.  What raises the reference m is applied to o after that.
+            static_assert(NS == 1);
+            char *sa = lds, *sb = lds + STAGE, *sc = lds + 2 * STAGE;
+            load();
+            write(t0, sa);
+            load();
+            write(t0 + 1, sb);
+            load();
+            u32x4 kb[STEPS], vb[STEPS];     // (two tiles of loads under way)
+            load_into(kb, vb);
+            __syncthreads();
+            constexpr int N = HD / 16, AHEAD = 8;
+            #pragma unroll
+            for (int j = 0; j < N; ++j) s[0] = mfma32<IO>(k_fragment<HD>(sa, lane, j), qf[j], j == 0 ? f32x16{} : s[0]);
+            softmax(t0, ok3, t0 < wf0 || t0 >= wf1 || ok3 != FULL);
+            const auto step = [&](int i, u32x4 (&ks)[STEPS], u32x4 (&vs)[STEPS]) __attribute__((always_inline)) {
+                clean(i + 2, ks, vs, ok1);
+                u32x4 f[AHEAD];
+                const auto read = [&](int j) {
+                    if (j < N) f[j % AHEAD] = k_fragment<HD>(sb, lane, j);
+                    else f[j % AHEAD] = v_fragment<HD>(sa + KT * RK, lane, (j - N) / (HD / 32), (j - N) % (HD / 32));
+                };
+                #pragma unroll
+                for (int j = 0; j < AHEAD; ++j) read(j);
+                #pragma unroll
+                for (int j = 0; j < N; ++j)
+                {
+                    __builtin_amdgcn_sched_barrier(0);
+                    s[0] = mfma32<IO>(f[j % AHEAD], qf[j], j == 0 ? f32x16{} : s[0]);
+                    read(j + AHEAD);
+                    if (j >= N - STEPS) write_step<HD, STEPS, LANES, RV>(ks, vs, j - (N - STEPS), tid, sc, sc + KT * RK);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                load_into(ks, vs);
+                const bool live = i + 1 < t1;
+                const uint64_t ok = live ? ok3 : 0;
+                float mx4[4], sum[4] = {}, alpha = 1.0f, base = 0.0f;
+                bool raised = false;
+                #pragma unroll
+                for (int j = 0; j < N; ++j)
+                {
+                    __builtin_amdgcn_sched_barrier(0);
+                    o[j % (HD / 32)] = mfma32<IO>(f[(N + j) % AHEAD], pf[j / (HD / 32)], o[j % (HD / 32)]);
+                    if (j + AHEAD < N) read(N + j + AHEAD);
+                    if (j == 1)
+                    {
+                        if (!live || i + 1 < wf0 || i + 1 >= wf1 || ok != FULL)
+                            mask_tile(s[0], tile_key(min(i + 1, t1 - 1)), half, row.p, a.window, a.sinks, (uint32_t)ok);
+                        #pragma unroll
+                        for (int e = 0; e < 8; ++e) mx4[e & 3] = e < 4 ? s[0][e] : fmaxf(mx4[e & 3], s[0][e]);
+                    }
+                    if (j == 2)
+                    {
+                        #pragma unroll
+                        for (int e = 8; e < 16; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], s[0][e]);
+                    }
+                    if (j == 3)
+                    {
+                        const float mx = max_xor32(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+                        raised = __any(mx > m + slack);
+                        const float mn = raised ? fmaxf(m, mx) : m;
+                        alpha = rescale_factor(m, mn, a.c);
+                        l = raised ? l * alpha : l;
+                        m = mn;
+                        base = exponent_base<IO>(m, a.c);
+                    }
+                    if (j >= 4 && j < 12)
+                    {
+                        #pragma unroll
+                        for (int e = 2 * (j - 4); e < 2 * (j - 4) + 2; ++e)
+                        {
+                            s[0][e] = __builtin_amdgcn_exp2f(fmaf(s[0][e], a.c, base));
+                            sum[e & 3] += s[0][e];
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                #pragma unroll
+                for (int e = 0; e < 8; ++e) pf[e / 4][e % 4] = pack2<IO>(s[0][2 * e], s[0][2 * e + 1]);
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (raised)
+                {
+                    #pragma unroll
+                    for (int t = 0; t < HD / 32; ++t)
+                        #pragma unroll
+                        for (int e = 0; e < 16; ++e) o[t][e] *= alpha;
+                }
+                char* const st = sa;
+                sa = sb;
+                sb = sc;
+                sc = st;
+                __syncthreads();
+            };
+            for (int i = t0; i < t1; i += 2)
+            {
+                step(i, ks, vs);
+                if (i + 1 < t1) step(i + 1, kb, vb);
+            }
+        }
+        else
+        {
         // A slot's products: o += V P with V of stage v (if `step`), then the scores of the keys of stage k.  LDS reads run
         // 8 MFMAs ahead of their use, in this order exactly: left to itself the compiler reads just before it
         // multiplies, and waits for each read.
@@ -671,6 +782,7 @@ __global__ __launch_bounds__(WAVES * 64, HD == 256 ? 1 : 2) void k_attn_rows(Att
             sb = sc;
             sc = st;
             __syncthreads();
+        }
         }
         if (!late && WAVES == 8) __syncthreads();
         if (a.err && bad) *a.err = 1;
