@@ -615,7 +615,7 @@ EXL3R_API int exl3r_act_mul_had(int act, const void* x, const void* y, int in_dt
  *        reading KV head h / (num_heads_q / num_heads_kv).
  *   k_cache, v_cache, page_size, num_pages, block_table, max_blocks_per_seq: as exl3r_rope_paged_kv (16-byte
  *        aligned).  max_blocks_per_seq * page_size and bsz * seq_len * num_heads_q below 2^31, num_heads_kv * head_dim
- *        at most 2^22.
+ *        at most 2^22.  (Refused too: more than 2^23 workgroups, or 2^24 query rows with a workspace.)
  *   err_flag: NULL or a device int32; 1 is stored for a token whose position is negative or past its block table
  *        (it sees the keys that the table holds) and for a visible key whose page is outside [0, num_pages) (it is
  *        taken as not visible).
