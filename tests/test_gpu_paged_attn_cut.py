@@ -95,3 +95,17 @@ def test_a_larger_workspace_from_the_whole_table():
 def test_scales(seq, scale):
     a = build([300, 7], seq, 4, 2, 64, F16, 32, seed=45, std=0.5)
     compare(call(*a, scale=scale), exact(*a, scale=scale), f"scale {scale}")
+
+
+@pytest.mark.parametrize("lens,seq,hq,hk,hd,page,blocks", [
+    ([3, 200, 127, 0], 1, 8, 2, 128, 64, 2),        # sequences shorter than the prefix; 128 of it
+    ([100, 20], 20, 8, 2, 256, 16, 8),              # ... and rows for the other kernel
+    ([255], 1, 8, 2, 64, 64, 4),                    # a batch of one whose table is all prefix
+    ([200, 190], 50, 4, 1, 128, 32, 8),
+])
+def test_prefix_beyond_a_sequence(lens, seq, hq, hk, hd, page, blocks):
+    """A prefix that some sequences have not reached, and one that fills the table."""
+    shared = page * blocks
+    spare = 0 if max(lens) + seq <= shared else 1
+    a = build(lens, seq, hq, hk, hd, BF16, page, shared, seed=46, spare_blocks=spare, poison=False)
+    compare(call(*a, shared=shared), exact(*a), f"prefix of {shared}")
